@@ -1,8 +1,7 @@
 // Matrix product with bias, activation and residual: out = act2(act(a w^T + bias) + residual).
 //
-// The weights are the row operand of the matrix instruction.  Its result gives a lane the values of rows 8i + 4h + c (i, c = 0..3,
-// h = the lane's half) of one column; feature 16h + 4i + c of a block of 32 is put into that row, so a lane ends with 16
-// neighbouring features of one row of the result: whole 16-byte stores, and a bias and a residual that are read the same way.
+// The weights are the row operand of the matrix instruction, so that a lane ends with neighbouring features of one row of the
+// result: whole 16-byte stores, and a bias and a residual that are read the same way.
 #include "ops_common.h"
 
 namespace chip {
@@ -15,7 +14,7 @@ struct MatmulArgs {
     Act act, act2;
     int32_t res_float, out_float;
     int32_t tiles, tiles_m, tiles_n;  // of the result
-    int32_t by_rows;                  // neighbouring tiles share their rows; otherwise their features
+    int32_t band;                     // rows of tiles in a band
 };
 
 struct MatmulPlan {
@@ -24,9 +23,6 @@ struct MatmulPlan {
     int kernel;  // row of matmul_kernels; the one for any strides where pointers are not aligned
     int any;
 };
-
-// the feature, within a block of 32, whose weights are row r of the matrix instruction
-__device__ inline int matmul_feature(int r) { return 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3); }
 
 // 8 values of a row from k on, zeros from K on
 template <typename T>
@@ -83,18 +79,12 @@ __device__ inline void matmul_write(O* p, int valid, const float (&v)[N])
     }
 }
 
-// N neighbouring features from n0 on of row m
+// N neighbouring features from n0 on of row m, with their bias: the activations, the residual, the result
 template <typename T, int N>
 __device__ inline void matmul_finish(const MatmulArgs& a, float (&v)[N], int m, int n0, void* out)
 {
     const int valid = a.n - n0;
     if (m >= a.m || valid <= 0) return;
-    if (a.bias) {
-        float b[N];
-        matmul_read(a.bias + n0, valid, b);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += b[i];
-    }
     act_apply(v, a.act);
     if (a.residual) {
         float r[N];
@@ -110,33 +100,48 @@ __device__ inline void matmul_finish(const MatmulArgs& a, float (&v)[N], int m, 
     else matmul_write((T*)out + at, valid, v);
 }
 
-// Tiles are dealt to the accelerator dies in turn (workgroup i runs on die i % 8): each die gets a run of neighbouring tiles, whose
-// operands its own L2 then serves.
-__device__ inline int matmul_tile(const MatmulArgs& a, int i)
+// Tiles are dealt to the accelerator dies in turn (workgroup i runs on die i % 8): each die gets a run of neighbouring tiles.  A
+// run goes through bands of a.band rows of tiles, down each column of a band, so that the tiles that a die works on at a time are
+// a block whose operands its own L2 serves: 32 tiles in a row read 33 tiles' operands, 4 x 8 read 12.
+__device__ inline void matmul_place(const MatmulArgs& a, int i, int& tm, int& tn)
 {
     const int die = i & 7, each = a.tiles >> 3, more = a.tiles & 7;
-    return die * each + min(die, more) + (i >> 3);
+    const int tile = die * each + min(die, more) + (i >> 3);
+    const int band = tile / (a.band * a.tiles_n), in = tile - band * a.band * a.tiles_n;
+    const int rows = min(a.band, a.tiles_m - band * a.band);
+    tn = in / rows;
+    tm = band * a.band + in - tn * rows;
 }
 
-__device__ inline __amdgpu_buffer_rsrc_t matmul_rsrc(const void* p)
+// buffer descriptor: base, no stride, 2 GiB - 1 bytes
+__device__ inline v4i matmul_rsrc(const void* p)
 {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, 0x7fffffff, 0x00020000);
+    const uint64_t at = (uint64_t)p;
+    return v4i{__builtin_amdgcn_readfirstlane((int)at), __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff), 0x7fffffff, 0x00020000};
 }
 
-// lane t's 16 bytes at `offset` + `step` go to LDS at place t from `to` on
-__device__ inline void matmul_load_lds(__amdgpu_buffer_rsrc_t from, v4i* to, int offset, int step)
+__device__ inline uint32_t matmul_lds(const v4i* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) v4i*)p; }
+
+// Lane t's 16 bytes at `offset` + `step` go to LDS at place t from `to` on.  Written out because the compiler, where it issues this
+// load itself, waits for all loads under way in front of one of three LDS reads of a loop (1498 against 1090 us for 8192 x 8192 x
+// 8192).  It has no result in registers; matmul_arrive is what waits for it.
+__device__ inline void matmul_load_lds(v4i from, uint32_t to, int offset, int step)
 {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, offset, step, 0, 0);
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(offset), "s"(from), "s"(step) : "memory", "m0");
 }
 
-// all of this wave's loads have landed, then every wave's
+// all of this wave's loads have landed but the newest N, its LDS reads are done, and so for every wave
+template <int N>
 __device__ inline void matmul_arrive()
 {
-    // by builtins: the compiler knows then that nothing is under way, and waits for no loads of its own accord behind it
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);  // loads have landed, LDS reads are done
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+__device__ inline void matmul_meet()
+{
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // Few rows, or few tiles: 16 FT features x 16 PT rows to a workgroup, whose waves split K; both operands straight from memory into
@@ -148,8 +153,8 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_split_kernel(MatmulArgs a, 
     constexpr int TILE = 256 * FT * PT;
     __shared__ float sums[WAVES][TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
-    const int tile = matmul_tile(a, blockIdx.x);
-    const int tm = a.by_rows ? tile / a.tiles_n : tile % a.tiles_m, tn = a.by_rows ? tile % a.tiles_n : tile / a.tiles_m;
+    int tm, tn;
+    matmul_place(a, blockIdx.x, tm, tn);
     const int m0 = tm * 16 * PT, n0 = tn * 16 * FT;
     const T *xr[PT], *wr[FT];
 #pragma unroll
@@ -203,86 +208,128 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_split_kernel(MatmulArgs a, 
         for (int s = 1; s < WAVES; ++s)
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] += sums[s][at + i];
-        const int row = at / (16 * FT);
-        matmul_finish<T>(a, v, m0 + row, n0 + at - row * 16 * FT, out);
+        const int row = at / (16 * FT), n = n0 + at - row * 16 * FT;
+        if (a.bias && n < a.n) {
+            float b[N];
+            matmul_read(a.bias + n, a.n - n, b);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] += b[i];
+        }
+        matmul_finish<T>(a, v, m0 + row, n, out);
     }
 }
 
-// BM x BN of the result to a workgroup of WM x WN waves, MB x NB blocks of 32 x 32 to a wave; both operands come 64 deep into two
-// LDS buffers by direct loads, the next step's while one is multiplied: one barrier a step.  A row of 64 values is eight pieces
-// of 16 bytes; piece c of row r lies at place c ^ (r & 7), so that the eight lanes that LDS serves at a time read eight places.
-// Rows behind the last are the last one again; pieces behind K are asked for behind the buffer's end, which gives zeros.
-template <typename T, int WM, int WN, int MB, int NB>
-__global__ __launch_bounds__(64 * WM * WN) void matmul_tile_kernel(MatmulArgs a, const T* x, const T* w, void* out)
+// BM x BN of the result to a workgroup of WM x WN waves, 16 MB rows x 64 features to a wave.  Both operands come 64 deep into two LDS
+// buffers by direct loads, one step ahead of the one that is multiplied.  A row of 64 values is eight pieces of 16 bytes; piece c
+// of row r lies at place c ^ (r >> 1 & 7), so that the sixteen lanes that LDS serves at a time read all of its 64 banks.  Rows
+// behind the last are the last one again; pieces behind K are asked for behind the buffer's end, which gives zeros.
+// Row 16 t + r of a wave's 64 rows of weights is feature 16 (r / 4) + 4 t + r % 4 of its 64: the four results that the matrix
+// instruction leaves in a lane are neighbours, and so are those of the four blocks t: 16 features of one row of the result.
+template <typename T, int WM, int WN, int MB>
+__global__ __launch_bounds__(64 * WM * WN, 2) void matmul_tile_kernel(MatmulArgs a, const T* x, const T* w, void* out)
 {
     typedef typename vec8<T>::type V;
-    constexpr int WAVES = WM * WN, BM = WM * MB * 32, BN = WN * NB * 32;
-    constexpr int XL = BM / 8 / WAVES, WL = BN / 8 / WAVES;  // loads of a wave: 8 rows each
-    __shared__ v4i x0[BM * 8], x1[BM * 8], w0[BN * 8], w1[BN * 8];
+    constexpr int WAVES = WM * WN, BM = WM * MB * 16, BN = WN * 64, BK = 64;
+    constexpr int XL = (BM / 8 + WAVES - 1) / WAVES, WL = BN / 8 / WAVES;  // loads of a wave: 8 rows each
+    __shared__ v4i xt[2 * BM * 8], wt[2 * BN * 8];
+    const uint32_t xl = matmul_lds(xt), wl = matmul_lds(wt);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int half = lane >> 5, r = lane & 31;
-    const int tile = matmul_tile(a, blockIdx.x);
-    const int tm = a.by_rows ? tile / a.tiles_n : tile % a.tiles_m, tn = a.by_rows ? tile % a.tiles_n : tile / a.tiles_m;
+    const int q = lane >> 4, r = lane & 15;
+    int tm, tn;
+    matmul_place(a, blockIdx.x, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
-    const int steps = (a.k + 63) / 64, last = a.k - (steps - 1) * 64;  // values of the last step
+    const int steps = (a.k + BK - 1) / BK;
 
     const auto xs = matmul_rsrc(x + (int64_t)m0 * a.a_pitch), ws = matmul_rsrc(w + (int64_t)n0 * a.w_pitch);
     int xo[XL], wo[WL];
+    const int turn = lane >> 4;  // row / 2 of the lane's row in a load; loads start at multiples of 8, which count by bit 3 only
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
-        const int row = (wave * XL + i) * 8 + (lane >> 3), c = (lane & 7) ^ (row & 7);
-        xo[i] = min(row, a.m - 1 - m0) * (int)(a.a_pitch * 2) + 16 * c;
+        const int row = (i * WAVES + wave) * 8 + (lane >> 3);
+        xo[i] = min(row, a.m - 1 - m0) * (int)(a.a_pitch * 2) + 16 * ((lane & 7) ^ (row >> 1 & 7));
     }
 #pragma unroll
     for (int i = 0; i < WL; ++i) {
-        // row q of LDS has the feature that row q of the matrix instruction stands for
-        const int row = (wave * WL + i) * 8 + (lane >> 3), c = (lane & 7) ^ (row & 7);
-        wo[i] = min((row & ~31) + matmul_feature(row & 31), a.n - 1 - n0) * (int)(a.w_pitch * 2) + 16 * c;
+        const int row = (i * WAVES + wave) * 8 + (lane >> 3), b = row & 63;
+        const int feature = (row & ~63) + 16 * (b >> 2 & 3) + 4 * (b >> 4) + (b & 3);
+        wo[i] = min(feature, a.n - 1 - n0) * (int)(a.w_pitch * 2) + 16 * ((lane & 7) ^ (row >> 1 & 7));
     }
-    const int reach = 8 * ((lane & 7) ^ (lane >> 3));  // the first of this lane's eight values of a step: (row & 7) == lane >> 3
-    const auto load = [&](int step, v4i* xb, v4i* wb) {
-        const int behind = step == steps - 1 && reach >= last ? (int)0x80000000 : 0;
+    // every load of a wave starts at the same multiple of 8 modulo 16
+    const int piece = (lane & 7) ^ (turn | (wave & 1) << 2);
+    static_assert(WAVES % 2 == 0, "");
+    const auto load = [&](int step, int at) {
+        const int behind = step * BK + 8 * piece >= a.k ? (int)0x80000000 : 0;
 #pragma unroll
-        for (int i = 0; i < XL; ++i) matmul_load_lds(xs, xb + (wave * XL + i) * 64, xo[i] | behind, step * 128);
+        for (int i = 0; i < XL; ++i)
+            if (BM / 8 % WAVES == 0 || i * WAVES + wave < BM / 8)
+                matmul_load_lds(xs, xl + at * BM * 128 + (i * WAVES + wave) * 1024, xo[i] | behind, step * 2 * BK);
 #pragma unroll
-        for (int i = 0; i < WL; ++i) matmul_load_lds(ws, wb + (wave * WL + i) * 64, wo[i] | behind, step * 128);
+        for (int i = 0; i < WL; ++i) matmul_load_lds(ws, wl + at * BN * 128 + (i * WAVES + wave) * 1024, wo[i] | behind, step * 2 * BK);
     };
     const int wm = wave / WN, wn = wave - wm * WN;
-    v16f acc[NB][MB] = {};
-    const auto multiply = [&](const v4i* xb, const v4i* wb) {
+    v4f acc[4][MB] = {};
+    V xf[MB], wf[4];
+    const auto read = [&](int round, int at) {
+        const int place = (4 * round + q) ^ (r >> 1);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int place = (2 * s + half) ^ (r & 7);
-            V xf[MB], wf[NB];
+        for (int j = 0; j < 4; ++j) wf[j] = __builtin_bit_cast(V, wt[at * BN * 8 + (wn * 64 + j * 16 + r) * 8 + place]);
 #pragma unroll
-            for (int j = 0; j < NB; ++j) wf[j] = __builtin_bit_cast(V, wb[((wn * NB + j) * 32 + r) * 8 + place]);
-#pragma unroll
-            for (int i = 0; i < MB; ++i) xf[i] = __builtin_bit_cast(V, xb[((wm * MB + i) * 32 + r) * 8 + place]);
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int j = 0; j < NB; ++j) acc[j][i] = mfma32(wf[j], xf[i], acc[j][i]);
-        }
+        for (int i = 0; i < MB; ++i) xf[i] = __builtin_bit_cast(V, xt[at * BM * 8 + ((wm * MB + i) * 16 + r) * 8 + place]);
     };
-    load(0, x0, w0);
-    for (int step = 0; step < steps; step += 2) {
-        matmul_arrive();
-        if (step + 1 < steps) load(step + 1, x1, w1);
-        multiply(x0, w0);
-        if (step + 1 == steps) break;
-        matmul_arrive();
-        if (step + 2 < steps) load(step + 2, x0, w0);
-        multiply(x1, w1);
-    }
+    const auto multiply = [&]() {
 #pragma unroll
-    for (int i = 0; i < MB; ++i)
+        for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            float v[16];
-#pragma unroll
-            for (int l = 0; l < 16; ++l) v[l] = acc[j][i][l];
-            matmul_finish<T>(a, v, m0 + (wm * MB + i) * 32 + r, n0 + (wn * NB + j) * 32 + 16 * half, out);
+            for (int j = 0; j < 4; ++j) acc[j][i] = mfma16(wf[j], xf[i], acc[j][i]);
+    };
+    load(0, 0);
+    matmul_arrive<0>();
+    if constexpr (WAVES == 8) {
+        // The second half of the waves runs one phase behind the first: on every SIMD one wave multiplies while the other fetches
+        // its operands.  A step is two rounds of that.
+        const bool late = wave >= WAVES / 2;
+        if (late) matmul_meet();
+        for (int step = 0, at = 0; step < steps; ++step, at ^= 1) {
+            load(step + 1, at ^ 1);
+            read(0, at);
+            matmul_meet();
+            __builtin_amdgcn_s_setprio(1);
+            multiply();
+            __builtin_amdgcn_s_setprio(0);
+            matmul_meet();
+            read(1, at);
+            // all reads of this buffer are done and the next step's loads have landed where the late waves end this phase
+            if (late) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            matmul_meet();
+            __builtin_amdgcn_s_setprio(1);
+            multiply();
+            __builtin_amdgcn_s_setprio(0);
+            if (!late) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            matmul_meet();
         }
+        if (!late) matmul_meet();
+    } else {
+        // two workgroups share a CU: one multiplies while the other waits
+        for (int step = 0, at = 0; step < steps; ++step, at ^= 1) {
+            load(step + 1, at ^ 1);
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                read(s, at);
+                multiply();
+            }
+            matmul_arrive<0>();
+        }
+    }
+    const int n = n0 + wn * 64 + 16 * q;
+    float bias[16] = {};
+    if (a.bias && n < a.n) matmul_read(a.bias + n, a.n - n, bias);
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        float v[16];
+#pragma unroll
+        for (int l = 0; l < 16; ++l) v[l] = acc[l / 4][i][l % 4] + bias[l];
+        matmul_finish<T>(a, v, m0 + (wm * MB + i) * 16 + r, n, out);
+    }
 }
 
 struct MatmulKernel {
@@ -290,25 +337,28 @@ struct MatmulKernel {
     int rows, features, waves;
 };
 static const MatmulKernel matmul_kernels[] = {
-    {"matmul_tile<256x256>", 256, 256, 8}, {"matmul_tile<128x128>", 128, 128, 4},
+    {"matmul_tile<256x256>", 256, 256, 8}, {"matmul_tile<224x256>", 224, 256, 8}, {"matmul_tile<192x256>", 192, 256, 8}, {"matmul_tile<160x256>", 160, 256, 8},
+    {"matmul_tile<128x256>", 128, 256, 8}, {"matmul_tile<128x128>", 128, 128, 4},
     {"matmul_split<64x64>", 64, 64, 4}, {"matmul_split<64x32>", 64, 32, 8}, {"matmul_split<32x32>", 32, 32, 8},
     {"matmul_split<64x16>", 64, 16, 8}, {"matmul_split<32x16>", 32, 16, 16}, {"matmul_split<16x16>", 16, 16, 16},
 };
+enum { MM_256 = 0, MM_128x256 = 4, MM_128 = 5, MM_64 = 6, MM_64x32, MM_32, MM_64x16, MM_32x16, MM_16 };
 
 static int64_t matmul_count(int m, int n, const MatmulKernel& k) { return (int64_t)((m + k.rows - 1) / k.rows) * ((n + k.features - 1) / k.features); }
 
 // whole: rows of 16-byte pieces, which the direct loads into LDS need
 static int matmul_choose(int m, int n, int k, bool whole, int cus)
 {
+    if (const char* f = getenv("MMF")) return atoi(f);
     const auto full = [&](int row) { return matmul_count(m, n, matmul_kernels[row]) >= cus; };
-    if (whole && full(0)) return 0;
-    if (whole && full(1)) return 1;
-    if (full(2)) return 2;
-    if (m <= 16) return 7;
-    if (m <= 32) return 6;
-    if (full(3)) return 3;
-    if (m > 64 || full(4)) return 4;
-    return 5;
+    if (whole && full(MM_256)) return MM_256;
+    if (whole && full(MM_128)) return MM_128;
+    if (full(MM_64)) return MM_64;
+    if (m <= 16) return MM_16;
+    if (m <= 32) return MM_32x16;
+    if (full(MM_64x32)) return MM_64x32;
+    if (m > 64 || full(MM_32)) return MM_32;
+    return MM_64x16;
 }
 
 static void matmul_tiles(MatmulArgs& a, const MatmulKernel& k)
@@ -316,8 +366,7 @@ static void matmul_tiles(MatmulArgs& a, const MatmulKernel& k)
     const int64_t tiles = matmul_count(a.m, a.n, k);
     CHIP_REQUIRE(tiles < (1ll << 31), CLDNN_HIP_UNSUPPORTED_SIZE, "matmul: too large");
     a.tiles = (int32_t)tiles, a.tiles_m = (a.m + k.rows - 1) / k.rows, a.tiles_n = (a.n + k.features - 1) / k.features;
-    // neighbouring tiles share what is larger
-    a.by_rows = a.m >= a.n;
+    a.band = 8;
 }
 
 MatmulPlan* matmul_plan(const cldnn_hip_engine_s& e, const cldnn_hip_matmul_desc& d, cldnn_hip_operator_info& info)
@@ -372,13 +421,17 @@ void matmul_launch(hipStream_t s, const MatmulPlan& p, void* workspace, const vo
         matmul_tiles(a, kernel);
         const auto launch = [&](auto f) { hipLaunchKernelGGL(f, dim3(a.tiles), dim3(64 * kernel.waves), 0, s, a, (const T*)x, (const T*)w, out); };
         switch (row) {
-        case 0: launch(matmul_tile_kernel<T, 2, 4, 4, 2>); break;
-        case 1: launch(matmul_tile_kernel<T, 2, 2, 2, 2>); break;
-        case 2: launch(matmul_split_kernel<T, 4, 4, 2, 4>); break;
-        case 3: launch(matmul_split_kernel<T, 2, 4, 3, 8>); break;
-        case 4: launch(matmul_split_kernel<T, 2, 2, 4, 8>); break;
-        case 5: launch(matmul_split_kernel<T, 1, 4, 4, 8>); break;
-        case 6: launch(matmul_split_kernel<T, 1, 2, 5, 16>); break;
+        case MM_256: launch(matmul_tile_kernel<T, 2, 4, 8>); break;
+        case MM_256 + 1: launch(matmul_tile_kernel<T, 2, 4, 7>); break;
+        case MM_256 + 2: launch(matmul_tile_kernel<T, 2, 4, 6>); break;
+        case MM_256 + 3: launch(matmul_tile_kernel<T, 2, 4, 5>); break;
+        case MM_128x256: launch(matmul_tile_kernel<T, 2, 4, 4>); break;
+        case MM_128: launch(matmul_tile_kernel<T, 2, 2, 4>); break;
+        case MM_64: launch(matmul_split_kernel<T, 4, 4, 2, 4>); break;
+        case MM_64x32: launch(matmul_split_kernel<T, 2, 4, 3, 8>); break;
+        case MM_32: launch(matmul_split_kernel<T, 2, 2, 4, 8>); break;
+        case MM_64x16: launch(matmul_split_kernel<T, 1, 4, 4, 8>); break;
+        case MM_32x16: launch(matmul_split_kernel<T, 1, 2, 5, 16>); break;
         default: launch(matmul_split_kernel<T, 1, 1, 8, 16>);
         }
     });
