@@ -17,11 +17,14 @@ struct MatmulArgs {
     int32_t band;                     // rows of tiles in a band
 };
 
+constexpr int64_t MATMUL_PACK = 200ll << 20;  // products from which unaligned operands are copied
+
 struct MatmulPlan {
     MatmulArgs a;
     int dt;
     int kernel;  // row of matmul_kernels; the one for any strides where pointers are not aligned
     int any;
+    int pieces;  // > 0: the operands are copied into rows of so many 16-byte pieces first
 };
 
 // 8 values of a row from k on, zeros from K on
@@ -225,20 +228,21 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_split_kernel(MatmulArgs a, 
 // behind the last are the last one again; pieces behind K are asked for behind the buffer's end, which gives zeros.
 // Row 16 t + r of a wave's 64 rows of weights is feature 16 (r / 4) + 4 t + r % 4 of its 64: the four results that the matrix
 // instruction leaves in a lane are neighbours, and so are those of the four blocks t: 16 features of one row of the result.
-template <typename T, int WM, int WN, int MB>
-__global__ __launch_bounds__(64 * WM * WN, 2) void matmul_tile_kernel(MatmulArgs a, const T* x, const T* w, void* out)
+template <typename T, int WM, int WN, int MB, int ST, int KG>
+__global__ __launch_bounds__(64 * WM * WN * KG, KG > 2 ? KG : 2) void matmul_tile_kernel(MatmulArgs a, const T* x, const T* w, void* out)
 {
     typedef typename vec8<T>::type V;
     constexpr int WAVES = WM * WN, BM = WM * MB * 16, BN = WN * 64, BK = 64;
     constexpr int XL = (BM / 8 + WAVES - 1) / WAVES, WL = BN / 8 / WAVES;  // loads of a wave: 8 rows each
-    __shared__ v4i xt[2 * BM * 8], wt[2 * BN * 8];
+    __shared__ v4i lds[KG * ST * (BM + BN) * 8];
+    const int lane = threadIdx.x & 63, every = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = every / WAVES, wave = every - group * WAVES;
+    const v4i *xt = lds + group * ST * (BM + BN) * 8, *wt = xt + ST * BM * 8;
     const uint32_t xl = matmul_lds(xt), wl = matmul_lds(wt);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, r = lane & 15;
     int tm, tn;
     matmul_place(a, blockIdx.x, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
-    const int steps = (a.k + BK - 1) / BK;
+    const int steps = ((a.k + BK - 1) / BK + KG - 1) / KG;  // group g takes every KG-th step from the g-th on
 
     const auto xs = matmul_rsrc(x + (int64_t)m0 * a.a_pitch), ws = matmul_rsrc(w + (int64_t)n0 * a.w_pitch);
     int xo[XL], wo[WL];
@@ -258,6 +262,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_tile_kernel(MatmulArgs
     const int piece = (lane & 7) ^ (turn | (wave & 1) << 2);
     static_assert(WAVES % 2 == 0, "");
     const auto load = [&](int step, int at) {
+        step = step * KG + group;
         const int behind = step * BK + 8 * piece >= a.k ? (int)0x80000000 : 0;
 #pragma unroll
         for (int i = 0; i < XL; ++i)
@@ -282,9 +287,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_tile_kernel(MatmulArgs
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[j][i] = mfma16(wf[j], xf[i], acc[j][i]);
     };
-    load(0, 0);
-    matmul_arrive<0>();
     if constexpr (WAVES == 8) {
+        load(0, 0);
+        matmul_arrive<0>();
         // The second half of the waves runs one phase behind the first: on every SIMD one wave multiplies while the other fetches
         // its operands.  A step is two rounds of that.
         const bool late = wave >= WAVES / 2;
@@ -309,18 +314,52 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_tile_kernel(MatmulArgs
         }
         if (!late) matmul_meet();
     } else {
-        // two workgroups share a CU: one multiplies while the other waits
-        for (int step = 0, at = 0; step < steps; ++step, at ^= 1) {
-            load(step + 1, at ^ 1);
+        // ST - 1 steps under way; what covers a wave's waits is another workgroup on its CU
+        static_assert(BM / 8 % WAVES == 0, "as many loads of every wave");
+#pragma unroll
+        for (int i = 0; i + 1 < ST; ++i) load(i, i);
+        for (int step = 0, at = 0, to = ST - 1; step < steps; ++step) {
+            matmul_arrive<(ST - 2) * (XL + WL)>();
+            load(step + ST - 1, to);
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 read(s, at);
                 multiply();
             }
-            matmul_arrive<0>();
+            to = at;
+            at = at + 1 == ST ? 0 : at + 1;
         }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
     const int n = n0 + wn * 64 + 16 * q;
+    if constexpr (KG > 1) {
+        // the groups' sums meet in LDS, in the order of the groups: group g finishes every KG-th block of rows
+        static_assert(KG * WAVES * MB * 256 <= KG * ST * (BM + BN) * 8 && (KG - 1) * MB >= 1, "the sums fit where the operands were");
+        asm volatile("s_barrier" ::: "memory");
+        v4f* sums = (v4f*)lds;
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sums[(((group * WAVES + wave) * MB + i) * 4 + j) * 64 + lane] = acc[j][i];
+        __syncthreads();
+        for (int i = group; i < MB; i += KG) {
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v4f t = sums[((wave * MB + i) * 4 + j) * 64 + lane];
+#pragma unroll
+                for (int g = 1; g < KG; ++g) t += sums[(((g * WAVES + wave) * MB + i) * 4 + j) * 64 + lane];
+#pragma unroll
+                for (int l = 0; l < 4; ++l) v[4 * j + l] = t[l];
+            }
+            float bias[16] = {};
+            if (a.bias && n < a.n) matmul_read(a.bias + n, a.n - n, bias);
+#pragma unroll
+            for (int l = 0; l < 16; ++l) v[l] += bias[l];
+            matmul_finish<T>(a, v, m0 + (wm * MB + i) * 16 + r, n, out);
+        }
+        return;
+    }
     float bias[16] = {};
     if (a.bias && n < a.n) matmul_read(a.bias + n, a.n - n, bias);
 #pragma unroll
@@ -332,33 +371,50 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_tile_kernel(MatmulArgs
     }
 }
 
+// Operands whose rows are no whole 16-byte pieces, copied into rows that are, zeros behind K: row i of a, then row j of weights.
+template <typename T>
+__global__ __launch_bounds__(256) void matmul_pack_kernel(MatmulArgs a, const T* x, const T* w, v4i* to, int pieces)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / pieces;
+    const int k = (int)(i - row * pieces) * 8;
+    if (row >= a.m + a.n) return;
+    to[i] = matmul_load8(row < a.m ? x + row * a.a_pitch : w + (row - a.m) * a.w_pitch, k, a.k);
+}
+
 struct MatmulKernel {
     const char* name;
     int rows, features, waves;
 };
+enum { MM_256, MM_224, MM_192, MM_128, MM_64x128, MM_64, MM_32, MM_ANY_64, MM_ANY_32, MM_16 };
 static const MatmulKernel matmul_kernels[] = {
-    {"matmul_tile<256x256>", 256, 256, 8}, {"matmul_tile<224x256>", 224, 256, 8}, {"matmul_tile<192x256>", 192, 256, 8}, {"matmul_tile<160x256>", 160, 256, 8},
-    {"matmul_tile<128x256>", 128, 256, 8}, {"matmul_tile<128x128>", 128, 128, 4},
-    {"matmul_split<64x64>", 64, 64, 4}, {"matmul_split<64x32>", 64, 32, 8}, {"matmul_split<32x32>", 32, 32, 8},
-    {"matmul_split<64x16>", 64, 16, 8}, {"matmul_split<32x16>", 32, 16, 16}, {"matmul_split<16x16>", 16, 16, 16},
+    {"matmul_tile<256x256>", 256, 256, 8}, {"matmul_tile<224x256>", 224, 256, 8}, {"matmul_tile<192x256>", 192, 256, 8},
+    {"matmul_tile<128x128>", 128, 128, 4}, {"matmul_tile<64x128>", 64, 128, 4}, {"matmul_tile<64x64,k2>", 64, 64, 8}, {"matmul_tile<32x64,k4>", 32, 64, 8},
+    {"matmul_split<64x64>", 64, 64, 4}, {"matmul_split<32x32>", 32, 32, 8}, {"matmul_split<16x16>", 16, 16, 16},
 };
-enum { MM_256 = 0, MM_128x256 = 4, MM_128 = 5, MM_64 = 6, MM_64x32, MM_32, MM_64x16, MM_32x16, MM_16 };
 
 static int64_t matmul_count(int m, int n, const MatmulKernel& k) { return (int64_t)((m + k.rows - 1) / k.rows) * ((n + k.features - 1) / k.features); }
 
 // whole: rows of 16-byte pieces, which the direct loads into LDS need
-static int matmul_choose(int m, int n, int k, bool whole, int cus)
+static int matmul_choose(int m, int n, bool whole, int cus)
 {
-    if (const char* f = getenv("MMF")) return atoi(f);
-    const auto full = [&](int row) { return matmul_count(m, n, matmul_kernels[row]) >= cus; };
-    if (whole && full(MM_256)) return MM_256;
-    if (whole && full(MM_128)) return MM_128;
-    if (full(MM_64)) return MM_64;
-    if (m <= 16) return MM_16;
-    if (m <= 32) return MM_32x16;
-    if (full(MM_64x32)) return MM_64x32;
-    if (m > 64 || full(MM_32)) return MM_32;
-    return MM_64x16;
+    const auto tiles = [&](int row) { return matmul_count(m, n, matmul_kernels[row]); };
+    const auto rounds = [&](int row) { return (tiles(row) + cus - 1) / cus; };
+    // Few tiles of any size: the smallest, whose 16 waves split K.  (us, against 32 x 64 tiles: 1 x 2048 -> 1000 4.7 and 7.0, 64 x 2048
+    // -> 1000 6.0 and 7.0; at twice as many tiles, 32 x 1024 -> 4096, 6.0 and 5.2)
+    if (tiles(MM_16) * 4 <= cus * 5) return MM_16;
+    if (!whole) return tiles(MM_ANY_64) >= cus ? MM_ANY_64 : MM_ANY_32;
+    if (tiles(MM_128) * 4 >= cus * 5) {
+        // A CU's time by the rows of its 256 features, which the smaller tiles fetch more operands for: measured at 8192 x 8192 x
+        // 8192, per row of a round, 1 / 1.02 / 1.11 / 1.22 (809 us, 902, 1010, 991).  25088 x 4096 -> 1024: 222, 210, 287 and 268 us.
+        const int kernel[] = {MM_256, MM_224, MM_192, MM_128};
+        const double time[] = {rounds(MM_256) * 256.0, rounds(MM_224) * 224 * 1.04, rounds(MM_192) * 192 * 1.12, rounds(MM_128) * 64 * 1.22};
+        return kernel[std::min_element(time, time + 4) - time];
+    }
+    // Fewer: what leaves no CU idle and pays the fewest trips to memory one behind the other.  (3136 x 512 -> 512: 128 x 128 8.8 us,
+    // 64 x 128 6.1, 64 x 64 9.1; 1024 x 1024 -> 1024: 13.3, 8.3, 6.6, 32 x 64 10.1; 196 x 1024 -> 2048: 12.3, 8.1, 6.2, 5.2)
+    if (tiles(MM_64x128) * 4 >= cus * 3) return MM_64x128;
+    if (tiles(MM_64) * 4 >= cus * 3) return MM_64;
+    return MM_32;
 }
 
 static void matmul_tiles(MatmulArgs& a, const MatmulKernel& k)
@@ -396,11 +452,19 @@ MatmulPlan* matmul_plan(const cldnn_hip_engine_s& e, const cldnn_hip_matmul_desc
     plan->dt = d.dtype;
     const int64_t out_size = a.out_float ? 4 : 2, res_size = !a.residual ? 0 : a.res_float ? 4 : 2;
     const int cus = e.props.multiProcessorCount;
-    plan->kernel = matmul_choose(d.m, d.n, d.k, d.k % 8 == 0 && a.a_pitch % 8 == 0 && a.w_pitch % 8 == 0 && std::max(a.a_pitch, a.w_pitch) < (1 << 21), cus);
-    plan->any = matmul_choose(d.m, d.n, d.k, false, cus);
+    const bool whole = d.k % 8 == 0 && a.a_pitch % 8 == 0 && a.w_pitch % 8 == 0 && std::max(a.a_pitch, a.w_pitch) < (1 << 21);
+    plan->kernel = matmul_choose(d.m, d.n, whole, cus);
+    plan->any = matmul_choose(d.m, d.n, false, cus);
+    // The copy costs a launch and two trips of the operands, the kernels for any rows 5 times the tiles' time from there on (4000 x 255
+    // -> 1000: 41 us without it, 10 with).
+    if (!whole && plan->any != MM_16 && (int64_t)d.m * d.n * d.k >= MATMUL_PACK && d.k < (1 << 20)) {
+        plan->pieces = (d.k + 7) / 8;
+        plan->kernel = matmul_choose(d.m, d.n, true, cus);
+    }
     const MatmulKernel& kernel = matmul_kernels[plan->kernel];
     matmul_tiles(a, kernel);
-    info.launches = 1, info.block = 64 * kernel.waves, info.grid = a.tiles;
+    info.launches = plan->pieces ? 2 : 1, info.block = 64 * kernel.waves, info.grid = a.tiles;
+    info.workspace_bytes = ((int64_t)d.m + d.n) * plan->pieces * 16;
     info.ops = 2ll * d.m * d.n * d.k;
     info.bytes = 2 * ((int64_t)d.m * d.k + (int64_t)d.n * d.k) + (d.has_bias ? 4ll * d.n : 0) + (int64_t)d.m * d.n * (out_size + res_size);
     snprintf(info.kernel_name, sizeof info.kernel_name, "%s", kernel.name);
@@ -416,22 +480,27 @@ void matmul_launch(hipStream_t s, const MatmulPlan& p, void* workspace, const vo
     if (a.residual) check_aligned(residual, a.res_float ? 4 : 2, "residual"), a.residual = residual;
     with_half(p.dt, [&](auto t) {
         typedef decltype(t) T;
-        const int row = (((uintptr_t)x | (uintptr_t)w) & 15) == 0 ? p.kernel : p.any;
+        const void *xa = x, *wa = w;
+        if (p.pieces) {
+            const int64_t blocks = (((int64_t)a.m + a.n) * p.pieces + 255) / 256;
+            hipLaunchKernelGGL((matmul_pack_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a, (const T*)x, (const T*)w, (v4i*)workspace, p.pieces);
+            a.a_pitch = a.w_pitch = a.k = 8 * p.pieces;
+            xa = workspace, wa = (const v4i*)workspace + (int64_t)a.m * p.pieces;
+        }
+        const int row = (((uintptr_t)xa | (uintptr_t)wa) & 15) == 0 ? p.kernel : p.any;
         const MatmulKernel& kernel = matmul_kernels[row];
         matmul_tiles(a, kernel);
-        const auto launch = [&](auto f) { hipLaunchKernelGGL(f, dim3(a.tiles), dim3(64 * kernel.waves), 0, s, a, (const T*)x, (const T*)w, out); };
+        const auto launch = [&](auto f) { hipLaunchKernelGGL(f, dim3(a.tiles), dim3(64 * kernel.waves), 0, s, a, (const T*)xa, (const T*)wa, out); };
         switch (row) {
-        case MM_256: launch(matmul_tile_kernel<T, 2, 4, 8>); break;
-        case MM_256 + 1: launch(matmul_tile_kernel<T, 2, 4, 7>); break;
-        case MM_256 + 2: launch(matmul_tile_kernel<T, 2, 4, 6>); break;
-        case MM_256 + 3: launch(matmul_tile_kernel<T, 2, 4, 5>); break;
-        case MM_128x256: launch(matmul_tile_kernel<T, 2, 4, 4>); break;
-        case MM_128: launch(matmul_tile_kernel<T, 2, 2, 4>); break;
-        case MM_64: launch(matmul_split_kernel<T, 4, 4, 2, 4>); break;
-        case MM_64x32: launch(matmul_split_kernel<T, 2, 4, 3, 8>); break;
-        case MM_32: launch(matmul_split_kernel<T, 2, 2, 4, 8>); break;
-        case MM_64x16: launch(matmul_split_kernel<T, 1, 4, 4, 8>); break;
-        case MM_32x16: launch(matmul_split_kernel<T, 1, 2, 5, 16>); break;
+        case MM_256: launch(matmul_tile_kernel<T, 2, 4, 8, 2, 1>); break;
+        case MM_224: launch(matmul_tile_kernel<T, 2, 4, 7, 2, 1>); break;
+        case MM_192: launch(matmul_tile_kernel<T, 2, 4, 6, 2, 1>); break;
+        case MM_128: launch(matmul_tile_kernel<T, 2, 2, 4, 2, 1>); break;
+        case MM_64x128: launch(matmul_tile_kernel<T, 2, 2, 2, 3, 1>); break;
+        case MM_64: launch(matmul_tile_kernel<T, 4, 1, 1, 4, 2>); break;
+        case MM_32: launch(matmul_tile_kernel<T, 2, 1, 1, 3, 4>); break;
+        case MM_ANY_64: launch(matmul_split_kernel<T, 4, 4, 2, 4>); break;
+        case MM_ANY_32: launch(matmul_split_kernel<T, 2, 2, 4, 8>); break;
         default: launch(matmul_split_kernel<T, 1, 1, 8, 16>);
         }
     });

@@ -37,16 +37,19 @@ struct Act {
     float m, n;
 };
 
-// erfc(|x|) exp-scaled to q = erfc(|x|): Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26 (error 1.5e-7).
-__device__ inline float erfc_abs(float x)
+// v P(Z <= v) = max(v, 0) - |v| P(Z > |v|), without a difference of near equals on either side.  P(Z > a) = erfc(a / sqrt 2) / 2 by
+// Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26 (error 1.5e-7), with the factors of 2 in its constants.
+__device__ inline float act_gelu(float v)
 {
-    const float a = __builtin_fabsf(x);
-    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, a, 1.0f));
-    float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-    p = __builtin_fmaf(p, t, 1.421413741f);
-    p = __builtin_fmaf(p, t, -0.284496736f);
-    p = __builtin_fmaf(p, t, 0.254829592f);
-    return p * t * __builtin_amdgcn_exp2f(-1.44269504f * a * a);
+    const float a = __builtin_fminf(__builtin_fabsf(v), 1e18f);  // infinity times no probability is no value
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678f, a, 1.0f));
+    float p = __builtin_fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+    p = __builtin_fmaf(p, t, 0.5f * 1.421413741f);
+    p = __builtin_fmaf(p, t, 0.5f * -0.284496736f);
+    p = __builtin_fmaf(p, t, 0.5f * 0.254829592f);
+    const float u = 0.84932180f * v;  // sqrt(log2(e) / 2)
+    const float q = p * t * __builtin_amdgcn_exp2f(-(u * u));
+    return __builtin_fmaf(-a, q, v < 0.0f ? 0.0f : v);
 }
 
 template <int KIND>
@@ -56,11 +59,7 @@ __device__ inline float act_one(float v, float m, float n)
     if constexpr (KIND == CLDNN_HIP_ACT_RELU_SLOPE) return v < 0.0f ? v * m : v;
     if constexpr (KIND == CLDNN_HIP_ACT_CLAMP) return v < m ? m : v > n ? n : v;
     if constexpr (KIND == CLDNN_HIP_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * v));
-    if constexpr (KIND == CLDNN_HIP_ACT_GELU) {
-        // v P(Z <= v): for v < 0 it is v erfc(|v| / sqrt 2) / 2 itself, without a difference of near equals
-        const float q = 0.5f * erfc_abs(v * 0.70710678f);
-        return v * (v < 0.0f ? q : 1.0f - q);
-    }
+    if constexpr (KIND == CLDNN_HIP_ACT_GELU) return act_gelu(v);
     if constexpr (KIND == CLDNN_HIP_ACT_GELU_TANH) {
         // (1 + tanh u) / 2 = 1 / (1 + exp(-2u)),  u = 0.79788456 (v + 0.044715 v^3)
         const float u = v * __builtin_fmaf(0.044715f * v, v, 1.0f);
