@@ -3,128 +3,218 @@
 // A wave has 32 rows: the queries of one key head, those of its sharing heads side by side.  It computes the scores transposed,
 // S^T = K Q^T, so that a row of the softmax lies in the registers of two lanes (32 apart), and the result transposed as well,
 // O^T = V^T P^T: the registers that S^T leaves in a lane are, as they lie, the operand that this second product wants, provided
-// that V's keys are taken in the same order: in a step of 16 keys lane half h has keys 4h..4h+3 and 8+4h..8+4h+3.
+// that V's keys are taken in the same order: in a step of 16 keys lane half h has keys 4h..4h+3 and 8+4h..8+4h+3.  That is what
+// the transposing LDS read gives, four keys of a value to a lane.
 // Values 16h + 4i + c of a block of 32 are put into row 8i + 4h + c of V^T, so a lane ends with 16 neighbouring values of its row.
-#include <cmath>
-
+//
+// The waves of a workgroup share tiles of 64 keys, which direct loads bring into LDS one tile ahead.  Where rows are few the keys
+// are split over workgroups (of one wave then), and a second kernel joins their parts.
 #include "ops_common.h"
 
 namespace chip {
 
 struct AttentionArgs {
     int32_t q_len, kv_len, kv_heads, group, head, rows;  // rows = q_len * group
-    float scale;  // without a bias times log2(e); with one the scores keep their own unit, where a bias of the lowest value is finite
+    int32_t blocks, splits, total;                       // workgroups along the rows, along the keys, in all
+    int32_t negative;                                    // scale < 0: the queries change their sign
+    float scale;   // of the scores, with a bias only: without one they stay as the product leaves them
+    float unit;    // of a score in powers of two.  With a bias log2(e): there a bias of the lowest value has to stay finite
+    float margin;  // 8 powers of two
     int64_t q_pb, q_pt, q_ph, k_pb, k_pt, k_ph, v_pb, v_pt, v_ph, o_pb, o_pt, o_ph, b_pb, b_ph, b_pq;
 };
 
 struct AttentionPlan {
     AttentionArgs a;
     int dt, batch, size, bias_dt, has_lengths;
+    int waves;
+    int far;  // keys too far apart for 32-bit offsets within a tile
 };
 
 constexpr int ATT_KEYS = 64;  // of a tile
+constexpr int ATT_ONE_WAVE = 128;  // largest head that a workgroup of one wave is made for: beyond, a CU holds one tile anyway
 
-// where 16-byte chunk c of a row of D values lies in a tile in LDS: 8 neighbouring rows have their chunks in 8 different places
+// Piece c (16 bytes) of row r of D values lies at place r * D / 8 + (c ^ att_turn(r)) of a tile in LDS: sixteen neighbouring rows
+// have a piece in all 64 banks, and so have four rows four neighbouring pieces, which the transposing read takes at a time.
 template <int D>
-__device__ inline int att_place(int row, int c)
+__device__ inline int att_turn(int r)
 {
-    constexpr int C = D / 8;
-    const int l = row * C + c;
-    return C % 8 == 0 ? l ^ (row & 7) : l ^ ((l >> 3) & 7);
+    if constexpr (D % 128 == 0) return (r & 1) << 3 | (r & 2) << 1 | (r >> 1 & 2) | (r >> 3 & 1);
+    if constexpr (D % 64 == 0) return (r << 1 & 4) | (r >> 1 & 2) | (r >> 3 & 1);
+    return r >> 2 & 3;
 }
 
-template <typename T, int D, typename B>
-__global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a, const T* q, const T* k, const T* v, const int32_t* lengths, const B* bias, T* out)
+template <typename T>
+__device__ inline v2i att_read_turned(const v4i* tile, int at)
+{
+    typedef short v4s __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) v4s* ptr;
+    return __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)((const __attribute__((address_space(3))) char*)tile + at)));
+}
+
+template <typename T, int D, typename B, int WAVES, bool FAR>
+__global__ __launch_bounds__(64 * WAVES, D <= 64 ? (std::is_same<B, void>::value ? 4 : 3) : D <= 160 ? 2 : 1) void attention_kernel(AttentionArgs a, const T* q, const T* k, const T* v, const int32_t* lengths, const B* bias, T* out, float* part)
 {
     typedef typename vec8<T>::type V8;
-    constexpr int C = D / 8, STEPS = D / 16, BLOCKS = D / 32;
+    constexpr int C = D / 8, STEPS = D / 16, BLOCKS = D / 32, TILE = ATT_KEYS * C, LOADS = C / WAVES;
     constexpr bool BIAS = !std::is_same<B, void>::value;
-    constexpr float unit = BIAS ? 1.44269504f : 1.0f;
-    __shared__ v4i kt[ATT_KEYS * C], vt[ATT_KEYS * C];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
-    const int b = blockIdx.z, kh = blockIdx.y;
-    const int row = min((int)(blockIdx.x * 128 + wave * 32 + col), a.rows - 1);
+    __shared__ v4i kt[2 * TILE], vt[2 * TILE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+    // as in the matrix product each die gets a run of workgroups: those of one head share its keys there
+    const int die = blockIdx.x & 7;
+    int block = die * (a.total >> 3) + min(die, a.total & 7) + (blockIdx.x >> 3);
+    const int pair_split = block / a.blocks;
+    block -= pair_split * a.blocks;
+    const int pair = pair_split / a.splits, split = pair_split - pair * a.splits, b = pair / a.kv_heads, kh = pair - b * a.kv_heads;
+    const int own = (block * WAVES + wave) * 32 + col, row = min(own, a.rows - 1);
     const int qi = row / a.group, h = kh * a.group + row - qi * a.group;
     const int length = lengths ? min(max(lengths[b], 0), a.kv_len) : a.kv_len;
+    const int tiles = (length + ATT_KEYS - 1) / ATT_KEYS;
+    const int first = (int)((int64_t)tiles * split / a.splits), last = (int)((int64_t)tiles * (split + 1) / a.splits);
     const int chunks = a.head / 8;
 
     V8 qf[STEPS];
     const T* qr = q + b * a.q_pb + qi * a.q_pt + h * a.q_ph;
+    const int sign = a.negative ? (int)0x80008000 : 0;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         const int c = 2 * s + half;
-        qf[s] = __builtin_bit_cast(V8, c < chunks ? *(const v4i*)(qr + 8 * c) : v4i{0, 0, 0, 0});
+        v4i x = {0, 0, 0, 0};
+        if (c < chunks) x = *(const v4i*)(qr + 8 * c) ^ v4i{sign, sign, sign, sign};
+        qf[s] = __builtin_bit_cast(V8, x);
     }
-    v16f o[BLOCKS] = {};
-    float most = -INFINITY, sum = 0.0f;
     const T* kb = k + b * a.k_pb + kh * a.k_ph;
     const T* vb = v + b * a.v_pb + kh * a.v_ph;
-    for (int key0 = 0; key0 < length; key0 += ATT_KEYS) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < ATT_KEYS * C; i += 256) {
-            const int key = i / C, c = i - key * C;
-            v4i kx = {0, 0, 0, 0}, vx = {0, 0, 0, 0};
-            if (key0 + key < length && c < chunks) {
-                kx = *(const v4i*)(kb + (int64_t)(key0 + key) * a.k_pt + 8 * c);
-                vx = *(const v4i*)(vb + (int64_t)(key0 + key) * a.v_pt + 8 * c);
+
+    // the tile's rows from a length on and the pieces behind the head are zeros
+    int ko[LOADS], vo[LOADS], key_of[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int at = (i * WAVES + wave) * 64 + lane, key = at / C, c = (at - key * C) ^ att_turn<D>(key);
+        key_of[i] = c < chunks ? key : 1 << 30;
+        if constexpr (!FAR) ko[i] = key * (int)(a.k_pt * 2) + 16 * c, vo[i] = key * (int)(a.v_pt * 2) + 16 * c;
+    }
+    const auto load = [&](int tile, int at) {
+        const int key0 = tile * ATT_KEYS;
+        if constexpr (FAR) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int to = (i * WAVES + wave) * 64 + lane, key = to / C, c = (to - key * C) ^ att_turn<D>(key);
+                const bool there = key_of[i] < length - key0;
+                kt[at * TILE + to] = there ? *(const v4i*)(kb + (int64_t)(key0 + key) * a.k_pt + 8 * c) : v4i{0, 0, 0, 0};
+                vt[at * TILE + to] = there ? *(const v4i*)(vb + (int64_t)(key0 + key) * a.v_pt + 8 * c) : v4i{0, 0, 0, 0};
             }
-            kt[att_place<D>(key, c)] = kx;
-            vt[att_place<D>(key, c)] = vx;
+        } else {
+            const v4i ks = buffer_of(kb + (int64_t)key0 * a.k_pt), vs = buffer_of(vb + (int64_t)key0 * a.v_pt);
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int behind = key_of[i] < length - key0 ? 0 : (int)0x80000000;
+                load_lds(ks, lds_address(kt) + at * TILE * 16 + (i * WAVES + wave) * 1024, ko[i] | behind, 0);
+                load_lds(vs, lds_address(vt) + at * TILE * 16 + (i * WAVES + wave) * 1024, vo[i] | behind, 0);
+            }
         }
-        __syncthreads();
+    };
+
+    // where the lane reads V: key 4 half + lane / 4 % 4 (+ 8) of a step, four values from 16 h + 4 i on
+    int vp[2][BLOCKS];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < BLOCKS; ++i) {
+            const int r = 8 * j + 4 * half + (lane >> 2 & 3), quad = (lane >> 4 & 1) * 4 + (lane & 3);
+            const int d = 32 * i + 16 * (quad & 1) + 4 * (quad >> 1);
+            vp[j][i] = (r * C + ((d / 8) ^ att_turn<D>(r))) * 16 + (d & 4) * 2;
+        }
+
+    v16f o[BLOCKS] = {};
+    float most = -INFINITY, sum = 0.0f;
+    if (first < last) load(first, 0);
+    for (int tile = first, at = 0; tile < last; ++tile, at ^= 1) {
+        if constexpr (FAR) __syncthreads();
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (tile + 1 < last) load(tile + 1, at ^ 1);
+        const v4i* kl = kt + at * TILE;
         v16f s[2] = {};
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i)
-                s[t] = mfma32(__builtin_bit_cast(V8, kt[att_place<D>(32 * t + col, 2 * i + half)]), qf[i], s[t]);
-        float top = most;
+            for (int t = 0; t < 2; ++t)
+                s[t] = mfma32(__builtin_bit_cast(V8, kl[(32 * t + col) * C + ((2 * i + half) ^ att_turn<D>(col))]), qf[i], s[t]);
+        const int key0 = tile * ATT_KEYS;
+        if constexpr (BIAS) {
+            const B* at_bias = bias + b * a.b_pb + h * a.b_ph + qi * a.b_pq;
+            typedef B any __attribute__((ext_vector_type(4), aligned(sizeof(B))));
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = key0 + 32 * t + 8 * (i / 4) + 4 * half + i % 4;
-                if constexpr (BIAS) {
-                    const int64_t at = b * a.b_pb + h * a.b_ph + qi * a.b_pq + min(key, a.kv_len - 1);
-                    s[t][i] = __builtin_fmaf(s[t][i], a.scale, (float)bias[at]);
-                } else s[t][i] *= a.scale;
-                s[t][i] = key < length ? s[t][i] : -INFINITY;
-                top = fmaxf(top, s[t][i]);
-            }
+                for (int i = 0; i < 4; ++i) {
+                    const int key = key0 + 32 * t + 8 * i + 4 * half;
+                    any x = {};
+                    if (key + 4 <= a.kv_len) x = *(const any*)(at_bias + key);
+                    else
+                        for (int j = 0; j < 3; ++j)
+                            if (key + j < a.kv_len) x[j] = at_bias[key + j];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[t][4 * i + j] = __builtin_fmaf(s[t][4 * i + j], a.scale, (float)x[j]);
+                }
+        }
+        if (key0 + ATT_KEYS > length)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (key0 + 32 * t + 8 * (i / 4) + 4 * half + i % 4 >= length) s[t][i] = -INFINITY;
+        float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float base = top == -INFINITY ? 0.0f : top;  // a row without a key so far
-        const float fade = __builtin_amdgcn_exp2f((most - base) * unit);
-        most = top;
-        sum *= fade;
+        // The maximum that the exponents are taken from follows when it is left behind by 2^8, which the sums and the operands of the
+        // second product hold without loss: after the first tiles hardly ever.
+        if (__any(top > most + a.margin)) {
+            const bool follow = top > most + a.margin;
+            const float fade = follow ? __builtin_amdgcn_exp2f((most - top) * a.unit) : 1.0f;
+            most = follow ? top : most;
+            sum *= fade;
 #pragma unroll
-        for (int i = 0; i < BLOCKS; ++i)
+            for (int i = 0; i < BLOCKS; ++i)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[i][j] *= fade;
+                for (int j = 0; j < 16; ++j) o[i][j] *= fade;
+        }
+        const float base = most == -INFINITY ? 0.0f : most;  // a row without a key so far
+        const float under = base * a.unit;
         V8 p[4];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float e = __builtin_amdgcn_exp2f((s[t][i] - base) * unit);
+                const float e = __builtin_amdgcn_exp2f(BIAS ? (s[t][i] - base) * a.unit : __builtin_fmaf(s[t][i], a.unit, -under));
                 sum += e;
                 p[2 * t + i / 8][i % 8] = (T)e;
             }
+        const v4i* vl = vt + at * TILE;
 #pragma unroll
         for (int st = 0; st < 4; ++st)
 #pragma unroll
             for (int i = 0; i < BLOCKS; ++i) {
-                const int d = 32 * i + 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);
-                V8 x;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int key = 16 * st + 8 * (j / 4) + 4 * half + j % 4;
-                    x[j] = ((const T*)&vt[att_place<D>(key, d / 8)])[d % 8];
-                }
-                o[i] = mfma32(x, p[st], o[i]);
+                const v2i lo = att_read_turned<T>(vl, vp[0][i] + st * 16 * C * 16), hi = att_read_turned<T>(vl, vp[1][i] + st * 16 * C * 16);
+                o[i] = mfma32(__builtin_bit_cast(V8, v4i{lo[0], lo[1], hi[0], hi[1]}), p[st], o[i]);
             }
     }
     sum += __shfl_xor(sum, 32);
-    if ((int)(blockIdx.x * 128 + wave * 32 + col) >= a.rows) return;
+    if (own >= a.rows) return;
+    if (a.splits > 1) {
+        const int64_t at = (int64_t)pair_split * a.rows + row;
+        float* to = part + at * a.head;
+#pragma unroll
+        for (int i = 0; i < BLOCKS; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int d = 32 * i + 16 * half + 4 * j;
+                if (d < a.head) *(v4f*)(to + d) = v4f{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
+            }
+        float2* ends = (float2*)(part + (int64_t)(a.total / a.blocks) * a.rows * a.head);
+        if (half == 0) ends[at] = make_float2(most, sum);
+        return;
+    }
     const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
     T* to = out + b * a.o_pb + qi * a.o_pt + h * a.o_ph;
 #pragma unroll
@@ -137,6 +227,40 @@ __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a, const T
             for (int l = 0; l < 8; ++l) x[l] = (T)(o[i][8 * j + l] * factor);
             if (d < a.head) *(V8*)(to + d) = x;
         }
+}
+
+// Joins the parts of a row: each is moved to the largest of their maxima.  One workgroup to a row of a head pair.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, const float* part, T* out)
+{
+    __shared__ float lds[256 + 4];
+    const int row = blockIdx.x, pair = blockIdx.y, b = pair / a.kv_heads, kh = pair - b * a.kv_heads, t = threadIdx.x;
+    const int64_t step = a.rows, at0 = (int64_t)pair * a.splits * a.rows + row;
+    const float2* ends = (const float2*)(part + (int64_t)(a.total / a.blocks) * a.rows * a.head);
+    float most = -INFINITY;
+    for (int s = t; s < a.splits; s += 256) most = fmaxf(most, ends[at0 + s * step].x);
+#pragma unroll
+    for (int i = 32; i; i >>= 1) most = fmaxf(most, __shfl_xor(most, i));
+    if ((t & 63) == 0) lds[256 + (t >> 6)] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(lds[256], lds[257]), fmaxf(lds[258], lds[259]));
+    if (most == -INFINITY) most = 0.0f;  // no key in any part
+    const int turns = 256 / a.head, turn = t / a.head, d = t - turn * a.head;
+    float value = 0.0f, sum = 0.0f;
+    if (turn < turns)
+        for (int s = turn; s < a.splits; s += turns) {
+            const float2 e = ends[at0 + s * step];
+            const float w = __builtin_amdgcn_exp2f((e.x - most) * a.unit);
+            sum = __builtin_fmaf(w, e.y, sum);
+            value = __builtin_fmaf(w, part[(at0 + s * step) * a.head + d], value);
+        }
+    __shared__ float sums[256];
+    lds[t] = value, sums[t] = sum;
+    __syncthreads();
+    if (t >= a.head) return;
+    for (int i = 1; i < turns; ++i) value += lds[i * a.head + t], sum += sums[i * a.head + t];
+    const int qi = row / a.group, h = kh * a.group + row - qi * a.group;
+    out[b * a.o_pb + qi * a.o_pt + h * a.o_ph + t] = (T)(sum == 0.0f ? 0.0f : value / sum);
 }
 
 AttentionPlan* attention_plan(const cldnn_hip_engine_s& e, const cldnn_hip_attention_desc& d, cldnn_hip_operator_info& info)
@@ -156,7 +280,11 @@ AttentionPlan* attention_plan(const cldnn_hip_engine_s& e, const cldnn_hip_atten
     const int64_t rows = (int64_t)d.q_len * a.group;
     CHIP_REQUIRE(rows < (1ll << 31) - 256 && d.batch <= 65535 && d.kv_heads <= 65535 && d.kv_len < (1 << 30), CLDNN_HIP_UNSUPPORTED_SIZE, "attention: too large");
     a.rows = (int32_t)rows;
-    a.scale = (d.bias_dtype == CLDNN_HIP_NO_TYPE ? 1.44269504f : 1.0f) * (d.scale != 0.0f ? d.scale : 1.0f / std::sqrt((float)d.head_size));
+    const float scale = d.scale != 0.0f ? d.scale : 1.0f / std::sqrt((float)d.head_size);
+    a.negative = scale < 0.0f;
+    a.scale = std::fabs(scale);
+    a.unit = 1.44269504f * (d.bias_dtype == CLDNN_HIP_NO_TYPE ? a.scale : 1.0f);
+    a.margin = 8.0f / a.unit;
     const auto strides = [&](int heads, int len, int64_t batch, int64_t token, int64_t head, int64_t& pb, int64_t& pt, int64_t& ph) {
         ph = head ? head : d.head_size;
         pt = token ? token : (int64_t)heads * d.head_size;
@@ -172,15 +300,26 @@ AttentionPlan* attention_plan(const cldnn_hip_engine_s& e, const cldnn_hip_atten
     a.b_pb = d.bias_batch_stride, a.b_ph = d.bias_head_stride, a.b_pq = d.bias_q_stride;
     plan->dt = d.dtype, plan->batch = d.batch, plan->bias_dt = d.bias_dtype, plan->has_lengths = d.has_key_lengths != 0;
     plan->size = d.head_size <= 32 ? 32 : d.head_size <= 64 ? 64 : d.head_size <= 96 ? 96 : d.head_size <= 128 ? 128 : d.head_size <= 160 ? 160 : 256;
+    plan->far = std::max(a.k_pt, a.v_pt) >= (1 << 24);
+    const int64_t pairs = (int64_t)d.batch * d.kv_heads;
+    const int cus = e.props.multiProcessorCount;
+    const bool few = rows * pairs < 64ll * cus;
+    plan->waves = few && plan->size <= ATT_ONE_WAVE ? 1 : 4;
+    a.blocks = (int)((rows + 32 * plan->waves - 1) / (32 * plan->waves));
+    a.splits = 1;
+    const int tiles = (d.kv_len + ATT_KEYS - 1) / ATT_KEYS;
+    if (few) a.splits = (int)std::max<int64_t>(1, std::min<int64_t>((2 * cus + a.blocks * pairs - 1) / (a.blocks * pairs), tiles / 2));
+    CHIP_REQUIRE(a.blocks * pairs * a.splits < (1ll << 31), CLDNN_HIP_UNSUPPORTED_SIZE, "attention: too large");
+    a.total = (int)(a.blocks * pairs * a.splits);
     const int64_t scores = (int64_t)d.batch * d.q_heads * d.q_len * d.kv_len;
     const int64_t bias_size = d.bias_dtype == CLDNN_HIP_NO_TYPE ? 0 : d.bias_dtype == CLDNN_HIP_F32 ? 4 : 2;
-    info.launches = 1, info.block = 256;
-    info.grid = (int)((rows + 127) / 128 * d.kv_heads * d.batch);
-    info.lds_bytes = 2 * ATT_KEYS * plan->size * 2;
+    info.launches = a.splits > 1 ? 2 : 1, info.block = 64 * plan->waves, info.grid = a.total;
+    info.lds_bytes = 4 * ATT_KEYS * plan->size * 2;
+    if (a.splits > 1) info.workspace_bytes = pairs * a.splits * rows * (d.head_size + 2) * 4;
     info.ops = 4 * scores * d.head_size;
     info.bytes = 4ll * d.batch * d.head_size * ((int64_t)d.q_len * d.q_heads + (int64_t)d.kv_len * d.kv_heads)
                  + bias_size * (a.b_pb ? d.batch : 1) * (a.b_ph ? d.q_heads : 1) * (a.b_pq ? d.q_len : 1) * (int64_t)d.kv_len;
-    snprintf(info.kernel_name, sizeof info.kernel_name, "attention<%d>", plan->size);
+    snprintf(info.kernel_name, sizeof info.kernel_name, "attention<%d%s%s>", plan->size, plan->waves == 1 ? ",one wave" : "", a.splits > 1 ? ",split keys" : "");
     return plan.release();
 }
 
@@ -194,15 +333,22 @@ void attention_launch(hipStream_t s, const AttentionPlan& p, void* workspace, co
     if (p.has_lengths) check_aligned(lengths, 4, "key_lengths");
     else lengths = nullptr;
     if (has_bias) check_aligned(bias, p.bias_dt == CLDNN_HIP_F32 ? 4 : 2, "bias");
-    const dim3 grid((unsigned)((a.rows + 127) / 128), a.kv_heads, p.batch);
     with_half(p.dt, [&](auto t) {
         typedef decltype(t) T;
         const auto launch = [&](auto d) {
             constexpr int D = decltype(d)::value;
-            const T *qt = (const T*)q, *kt = (const T*)k, *vt = (const T*)v;
-            if (!has_bias) hipLaunchKernelGGL((attention_kernel<T, D, void>), grid, dim3(256), 0, s, a, qt, kt, vt, lengths, (const void*)nullptr, (T*)out);
-            else if (p.bias_dt == CLDNN_HIP_F32) hipLaunchKernelGGL((attention_kernel<T, D, float>), grid, dim3(256), 0, s, a, qt, kt, vt, lengths, (const float*)bias, (T*)out);
-            else hipLaunchKernelGGL((attention_kernel<T, D, T>), grid, dim3(256), 0, s, a, qt, kt, vt, lengths, (const T*)bias, (T*)out);
+            const auto with = [&](auto* of) {
+                typedef typename std::remove_pointer<decltype(of)>::type B;
+                const auto go = [&](auto f) {
+                    hipLaunchKernelGGL(f, dim3(a.total), dim3(64 * p.waves), 0, s, a, (const T*)q, (const T*)k, (const T*)v, lengths, (const B*)bias, (T*)out, (float*)workspace);
+                };
+                if constexpr (D <= ATT_ONE_WAVE)
+                    if (p.waves == 1) return go(p.far ? attention_kernel<T, D, B, 1, true> : attention_kernel<T, D, B, 1, false>);
+                go(p.far ? attention_kernel<T, D, B, 4, true> : attention_kernel<T, D, B, 4, false>);
+            };
+            if (!has_bias) with((void*)nullptr);
+            else if (p.bias_dt == CLDNN_HIP_F32) with((float*)nullptr);
+            else with((T*)nullptr);
         };
         switch (p.size) {
         case 32: launch(std::integral_constant<int, 32>()); break;
@@ -212,6 +358,8 @@ void attention_launch(hipStream_t s, const AttentionPlan& p, void* workspace, co
         case 160: launch(std::integral_constant<int, 160>()); break;
         default: launch(std::integral_constant<int, 256>());
         }
+        if (a.splits > 1)
+            hipLaunchKernelGGL((attention_join_kernel<T>), dim3(a.rows, p.a.total / a.blocks / a.splits), dim3(256), 0, s, a, (const float*)workspace, (T*)out);
     });
     CHIP_CHECK(hipGetLastError());
 }

@@ -116,23 +116,6 @@ __device__ inline void matmul_place(const MatmulArgs& a, int i, int& tm, int& tn
     tm = band * a.band + in - tn * rows;
 }
 
-// buffer descriptor: base, no stride, 2 GiB - 1 bytes
-__device__ inline v4i matmul_rsrc(const void* p)
-{
-    const uint64_t at = (uint64_t)p;
-    return v4i{__builtin_amdgcn_readfirstlane((int)at), __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff), 0x7fffffff, 0x00020000};
-}
-
-__device__ inline uint32_t matmul_lds(const v4i* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) v4i*)p; }
-
-// Lane t's 16 bytes at `offset` + `step` go to LDS at place t from `to` on.  Written out because the compiler, where it issues this
-// load itself, waits for all loads under way in front of one of three LDS reads of a loop (1498 against 1090 us for 8192 x 8192 x
-// 8192).  It has no result in registers; matmul_arrive is what waits for it.
-__device__ inline void matmul_load_lds(v4i from, uint32_t to, int offset, int step)
-{
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(offset), "s"(from), "s"(step) : "memory", "m0");
-}
-
 // all of this wave's loads have landed but the newest N, its LDS reads are done, and so for every wave
 template <int N>
 __device__ inline void matmul_arrive()
@@ -237,14 +220,14 @@ __global__ __launch_bounds__(64 * WM * WN * KG, KG > 2 ? KG : 2) void matmul_til
     __shared__ v4i lds[KG * ST * (BM + BN) * 8];
     const int lane = threadIdx.x & 63, every = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = every / WAVES, wave = every - group * WAVES;
     const v4i *xt = lds + group * ST * (BM + BN) * 8, *wt = xt + ST * BM * 8;
-    const uint32_t xl = matmul_lds(xt), wl = matmul_lds(wt);
+    const uint32_t xl = lds_address(xt), wl = lds_address(wt);
     const int q = lane >> 4, r = lane & 15;
     int tm, tn;
     matmul_place(a, blockIdx.x, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
     const int steps = ((a.k + BK - 1) / BK + KG - 1) / KG;  // group g takes every KG-th step from the g-th on
 
-    const auto xs = matmul_rsrc(x + (int64_t)m0 * a.a_pitch), ws = matmul_rsrc(w + (int64_t)n0 * a.w_pitch);
+    const auto xs = buffer_of(x + (int64_t)m0 * a.a_pitch), ws = buffer_of(w + (int64_t)n0 * a.w_pitch);
     int xo[XL], wo[WL];
     const int turn = lane >> 4;  // row / 2 of the lane's row in a load; loads start at multiples of 8, which count by bit 3 only
 #pragma unroll
@@ -267,9 +250,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG, KG > 2 ? KG : 2) void matmul_til
 #pragma unroll
         for (int i = 0; i < XL; ++i)
             if (BM / 8 % WAVES == 0 || i * WAVES + wave < BM / 8)
-                matmul_load_lds(xs, xl + at * BM * 128 + (i * WAVES + wave) * 1024, xo[i] | behind, step * 2 * BK);
+                load_lds(xs, xl + at * BM * 128 + (i * WAVES + wave) * 1024, xo[i] | behind, step * 2 * BK);
 #pragma unroll
-        for (int i = 0; i < WL; ++i) matmul_load_lds(ws, wl + at * BN * 128 + (i * WAVES + wave) * 1024, wo[i] | behind, step * 2 * BK);
+        for (int i = 0; i < WL; ++i) load_lds(ws, wl + at * BN * 128 + (i * WAVES + wave) * 1024, wo[i] | behind, step * 2 * BK);
     };
     const int wm = wave / WN, wn = wave - wm * WN;
     v4f acc[4][MB] = {};

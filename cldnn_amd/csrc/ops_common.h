@@ -31,6 +31,25 @@ __device__ inline v16f mfma32(v8b a, v8b b, v16f c) { return __builtin_amdgcn_mf
 __device__ inline v4f mfma16(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ inline v4f mfma16(v8b a, v8b b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
+// ----------------------------------------------------------------------------- loads into LDS
+// buffer descriptor: base, no stride, 2 GiB - 1 bytes
+__device__ inline v4i buffer_of(const void* p)
+{
+    const uint64_t at = (uint64_t)p;
+    return v4i{__builtin_amdgcn_readfirstlane((int)at), __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff), 0x7fffffff, 0x00020000};
+}
+
+__device__ inline uint32_t lds_address(const v4i* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) v4i*)p; }
+
+// Lane t's 16 bytes at `offset` + `step` go to LDS at place t from `to` on.  Written out because the compiler, where it issues this
+// load itself, waits for all loads under way in front of one of three LDS reads of a loop (1498 against 1090 us for 8192 x 8192 x
+// 8192).  It has no result in registers; a wait for vmcnt, written out as well, is what it needs before anybody reads.
+// M0, which it sets, has no other user in these kernels: this device's LDS instructions do not read it, and no register is indexed.
+__device__ inline void load_lds(v4i from, uint32_t to, int offset, int step)
+{
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(offset), "s"(from), "s"(step) : "memory");
+}
+
 // ----------------------------------------------------------------------------- activations
 struct Act {
     int32_t kind;
