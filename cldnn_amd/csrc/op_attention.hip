@@ -51,12 +51,38 @@ __device__ inline v2i att_read_turned(const v4i* tile, int at)
     return __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)((const __attribute__((address_space(3))) char*)tile + at)));
 }
 
+// The largest of three.  Written out: fmaxf turns signalling NaNs of its operands quiet first, an instruction for each score.  `a`
+// has to depend on an ordinary instruction that read the last of the matrix instructions that b and c come from: the compiler
+// counts the wait states of their results for that one.
+__device__ inline float att_max(float a, float b, float c)
+{
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// f of a lane's value and that of the lane 32 apart
+template <typename F>
+__device__ inline float att_both(float x, F&& f)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+    return f(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
+
+// sum + a + b in one instruction, of probabilities as they are rounded: bf16 only, whose smallest values no sum misses
+__device__ inline float att_add(__bf16 a, __bf16 b, float sum)
+{
+    typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(v2b{a, b}, v2b{(__bf16)1.0f, (__bf16)1.0f}, sum, false);
+}
+__device__ inline float att_add(_Float16 a, _Float16 b, float sum) { return sum + (float)a + (float)b; }
+
 template <typename T, int D, typename B, int WAVES, bool FAR>
 __global__ __launch_bounds__(64 * WAVES, D <= 64 ? (std::is_same<B, void>::value ? 4 : 3) : D <= 160 ? 2 : 1) void attention_kernel(AttentionArgs a, const T* q, const T* k, const T* v, const int32_t* lengths, const B* bias, T* out, float* part)
 {
     typedef typename vec8<T>::type V8;
     constexpr int C = D / 8, STEPS = D / 16, BLOCKS = D / 32, TILE = ATT_KEYS * C, LOADS = C / WAVES;
-    constexpr bool BIAS = !std::is_same<B, void>::value;
+    constexpr bool BIAS = !std::is_same<B, void>::value, ROUNDED = std::is_same<T, __bf16>::value;
     __shared__ v4i kt[2 * TILE], vt[2 * TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
     // as in the matrix product each die gets a run of workgroups: those of one head share its keys there
@@ -165,8 +191,8 @@ __global__ __launch_bounds__(64 * WAVES, D <= 64 ? (std::is_same<B, void>::value
                     if (key0 + 32 * t + 8 * (i / 4) + 4 * half + i % 4 >= length) s[t][i] = -INFINITY;
         float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
-        top = fmaxf(top, __shfl_xor(top, 32));
+        for (int i = 1; i < 16; ++i) top = att_max(top, s[0][i], s[1][i]);
+        top = att_both(top, [](float x, float y) { return fmaxf(x, y); });
         // The maximum that the exponents are taken from follows when it is left behind by 2^8, which the sums and the operands of the
         // second product hold without loss: after the first tiles hardly ever.
         if (__any(top > most + a.margin)) {
@@ -187,9 +213,14 @@ __global__ __launch_bounds__(64 * WAVES, D <= 64 ? (std::is_same<B, void>::value
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float e = __builtin_amdgcn_exp2f(BIAS ? (s[t][i] - base) * a.unit : __builtin_fmaf(s[t][i], a.unit, -under));
-                sum += e;
+                if constexpr (!ROUNDED) sum += e;
                 p[2 * t + i / 8][i % 8] = (T)e;
             }
+        if constexpr (ROUNDED)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) sum = att_add(p[i][j], p[i][j + 1], sum);
         const v4i* vl = vt + at * TILE;
 #pragma unroll
         for (int st = 0; st < 4; ++st)
@@ -199,7 +230,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 64 ? (std::is_same<B, void>::value
                 o[i] = mfma32(__builtin_bit_cast(V8, v4i{lo[0], lo[1], hi[0], hi[1]}), p[st], o[i]);
             }
     }
-    sum += __shfl_xor(sum, 32);
+    sum = att_both(sum, [](float x, float y) { return x + y; });
     if (own >= a.rows) return;
     if (a.splits > 1) {
         const int64_t at = (int64_t)pair_split * a.rows + row;

@@ -127,7 +127,7 @@ cldnn_hip_status cldnn_hip_rotary_enqueue(cldnn_hip_operator op, const void* q_d
  * over the keys j < key_lengths[b] (clipped to 0..kv_len; all kv_len without lengths).  Keys and values at and behind a
  * length are never used, whatever their memory holds.  A row without a key, or with -infinity in all its scores, is
  * zeros.  The bias is ordinary arithmetic: -infinity takes a finite key out.  F16 or BF16; the softmax in 32 bits; the
- * probabilities are rounded to the data's type for the second product (their sum is not).
+ * probabilities are rounded to the data's type for the second product (and in BF16 their sum is that of the rounded ones).
  * head_size: a multiple of 8 up to 256; rows of q, k, v and out must be 16-byte aligned (pointers and strides). */
 typedef struct {
     int32_t batch, q_len, kv_len, q_heads, kv_heads, head_size;  /* q_heads a multiple of kv_heads */
