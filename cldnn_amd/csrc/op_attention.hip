@@ -160,11 +160,13 @@ __global__ __launch_bounds__(64 * WAVES, D <= 64 ? (std::is_same<B, void>::value
         if (tile + 1 < last) load(tile + 1, at ^ 1);
         const v4i* kl = kt + at * TILE;
         v16f s[2] = {};
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < STEPS; ++i)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
                 s[t] = mfma32(__builtin_bit_cast(V8, kl[(32 * t + col) * C + ((2 * i + half) ^ att_turn<D>(col))]), qf[i], s[t]);
+        __builtin_amdgcn_s_setprio(0);
         const int key0 = tile * ATT_KEYS;
         if constexpr (BIAS) {
             const B* at_bias = bias + b * a.b_pb + h * a.b_ph + qi * a.b_pq;
@@ -222,6 +224,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 64 ? (std::is_same<B, void>::value
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) sum = att_add(p[i][j], p[i][j + 1], sum);
         const v4i* vl = vt + at * TILE;
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int st = 0; st < 4; ++st)
 #pragma unroll
@@ -229,6 +232,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 64 ? (std::is_same<B, void>::value
                 const v2i lo = att_read_turned<T>(vl, vp[0][i] + st * 16 * C * 16), hi = att_read_turned<T>(vl, vp[1][i] + st * 16 * C * 16);
                 o[i] = mfma32(__builtin_bit_cast(V8, v4i{lo[0], lo[1], hi[0], hi[1]}), p[st], o[i]);
             }
+        __builtin_amdgcn_s_setprio(0);
     }
     sum = att_both(sum, [](float x, float y) { return x + y; });
     if (own >= a.rows) return;
@@ -336,6 +340,10 @@ AttentionPlan* attention_plan(const cldnn_hip_engine_s& e, const cldnn_hip_atten
     const int cus = e.props.multiProcessorCount;
     const bool few = rows * pairs < 64ll * cus;
     plan->waves = few && plan->size <= ATT_ONE_WAVE ? 1 : 4;
+    // Eight waves to a tile of keys where that leaves the fullest CU no more waves: half the trips into LDS (4096 x 4096 x 8 heads of
+    // 64, batch 4: 146 and 157 us with eight and four; one CU's share the other way round, batch 5: 209 and 194).
+    const auto fullest = [&](int waves) { return ((rows + 32 * waves - 1) / (32 * waves) * pairs + cus - 1) / cus * waves; };
+    if (!few && plan->size % 64 == 0 && plan->size <= 128 && fullest(8) * 95 < fullest(4) * 100) plan->waves = 8;
     a.blocks = (int)((rows + 32 * plan->waves - 1) / (32 * plan->waves));
     a.splits = 1;
     const int tiles = (d.kv_len + ATT_KEYS - 1) / ATT_KEYS;
@@ -375,6 +383,8 @@ void attention_launch(hipStream_t s, const AttentionPlan& p, void* workspace, co
                 };
                 if constexpr (D <= ATT_ONE_WAVE)
                     if (p.waves == 1) return go(p.far ? attention_kernel<T, D, B, 1, true> : attention_kernel<T, D, B, 1, false>);
+                if constexpr (D % 64 == 0 && D <= 128)
+                    if (p.waves == 8) return go(p.far ? attention_kernel<T, D, B, 8, true> : attention_kernel<T, D, B, 8, false>);
                 go(p.far ? attention_kernel<T, D, B, 4, true> : attention_kernel<T, D, B, 4, false>);
             };
             if (!has_bias) with((void*)nullptr);
