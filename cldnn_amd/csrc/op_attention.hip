@@ -264,38 +264,63 @@ __global__ __launch_bounds__(64 * WAVES, D <= 64 ? (std::is_same<B, void>::value
         }
 }
 
-// Joins the parts of a row: each is moved to the largest of their maxima.  One workgroup to a row of a head pair.
+// Joins the parts of a row: each is moved to the largest of their maxima.  One workgroup to a row of a head pair; four values to a
+// thread, so that few rounds of loads lie one behind the other (128 parts of a row of 128: 18 us with a value and 2 parts at a time).
+constexpr int ATT_JOIN = 512, ATT_MOST_SPLITS = 1024;
 template <typename T>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, const float* part, T* out)
+__global__ __launch_bounds__(ATT_JOIN) void attention_join_kernel(AttentionArgs a, const float* part, T* out)
 {
-    __shared__ float lds[256 + 4];
+    __shared__ float weight[ATT_MOST_SPLITS], both[2][ATT_JOIN / 64];
+    __shared__ v4f values[ATT_JOIN];
     const int row = blockIdx.x, pair = blockIdx.y, b = pair / a.kv_heads, kh = pair - b * a.kv_heads, t = threadIdx.x;
-    const int64_t step = a.rows, at0 = (int64_t)pair * a.splits * a.rows + row;
+    const int64_t at0 = (int64_t)pair * a.splits * a.rows + row;
     const float2* ends = (const float2*)(part + (int64_t)(a.total / a.blocks) * a.rows * a.head);
+    // the parts' values are asked for before their weights are known
+    const int lanes = a.head / 4, turns = ATT_JOIN / lanes, turn = t / lanes, d = (t - turn * lanes) * 4;
+    const bool live = turn < turns;
+    const auto value = [&](int s) { return live && s < a.splits ? *(const v4f*)(part + (at0 + (int64_t)s * a.rows) * a.head + d) : v4f{0, 0, 0, 0}; };
+    v4f first[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) first[i] = value(turn + i * turns);
+    float2 end[ATT_MOST_SPLITS / ATT_JOIN];
     float most = -INFINITY;
-    for (int s = t; s < a.splits; s += 256) most = fmaxf(most, ends[at0 + s * step].x);
+#pragma unroll
+    for (int i = 0; i < ATT_MOST_SPLITS / ATT_JOIN; ++i) {
+        const int s = t + i * ATT_JOIN;
+        end[i] = s < a.splits ? ends[at0 + (int64_t)s * a.rows] : make_float2(-INFINITY, 0.0f);
+        most = fmaxf(most, end[i].x);
+    }
 #pragma unroll
     for (int i = 32; i; i >>= 1) most = fmaxf(most, __shfl_xor(most, i));
-    if ((t & 63) == 0) lds[256 + (t >> 6)] = most;
+    if ((t & 63) == 0) both[0][t >> 6] = most;
     __syncthreads();
-    most = fmaxf(fmaxf(lds[256], lds[257]), fmaxf(lds[258], lds[259]));
+    for (int i = 0; i < ATT_JOIN / 64; ++i) most = fmaxf(most, both[0][i]);
     if (most == -INFINITY) most = 0.0f;  // no key in any part
-    const int turns = 256 / a.head, turn = t / a.head, d = t - turn * a.head;
-    float value = 0.0f, sum = 0.0f;
-    if (turn < turns)
-        for (int s = turn; s < a.splits; s += turns) {
-            const float2 e = ends[at0 + s * step];
-            const float w = __builtin_amdgcn_exp2f((e.x - most) * a.unit);
-            sum = __builtin_fmaf(w, e.y, sum);
-            value = __builtin_fmaf(w, part[(at0 + s * step) * a.head + d], value);
-        }
-    __shared__ float sums[256];
-    lds[t] = value, sums[t] = sum;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < ATT_MOST_SPLITS / ATT_JOIN; ++i) {
+        const float w = __builtin_amdgcn_exp2f((end[i].x - most) * a.unit);
+        if (t + i * ATT_JOIN < a.splits) weight[t + i * ATT_JOIN] = w;
+        sum = __builtin_fmaf(w, end[i].y, sum);
+    }
+#pragma unroll
+    for (int i = 32; i; i >>= 1) sum += __shfl_xor(sum, i);
+    if ((t & 63) == 0) both[1][t >> 6] = sum;
+    __syncthreads();
+    sum = 0.0f;
+    for (int i = 0; i < ATT_JOIN / 64; ++i) sum += both[1][i];
+    v4f v = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (live && turn + i * turns < a.splits) v += first[i] * weight[turn + i * turns];
+    for (int s = turn + 4 * turns; live && s < a.splits; s += turns) v += value(s) * weight[s];
+    values[t] = v;
     __syncthreads();
     if (t >= a.head) return;
-    for (int i = 1; i < turns; ++i) value += lds[i * a.head + t], sum += sums[i * a.head + t];
+    float x = 0.0f;
+    for (int i = 0; i < turns; ++i) x += ((const float*)values)[i * a.head + t];
     const int qi = row / a.group, h = kh * a.group + row - qi * a.group;
-    out[b * a.o_pb + qi * a.o_pt + h * a.o_ph + t] = (T)(sum == 0.0f ? 0.0f : value / sum);
+    out[b * a.o_pb + qi * a.o_pt + h * a.o_ph + t] = (T)(sum == 0.0f ? 0.0f : x / sum);
 }
 
 AttentionPlan* attention_plan(const cldnn_hip_engine_s& e, const cldnn_hip_attention_desc& d, cldnn_hip_operator_info& info)
@@ -347,7 +372,10 @@ AttentionPlan* attention_plan(const cldnn_hip_engine_s& e, const cldnn_hip_atten
     a.blocks = (int)((rows + 32 * plan->waves - 1) / (32 * plan->waves));
     a.splits = 1;
     const int tiles = (d.kv_len + ATT_KEYS - 1) / ATT_KEYS;
-    if (few) a.splits = (int)std::max<int64_t>(1, std::min<int64_t>((2 * cus + a.blocks * pairs - 1) / (a.blocks * pairs), tiles / 2));
+    // Two tiles at least to a part, parts for two workgroups to a CU.  The second kernel costs as much as four tiles one behind the
+    // other.  (us, parts of 2, 4, 8 tiles: 1 query, 4096 keys, 8 key heads of 128: 12.6, 15.4, 22.3; all in one: 115.  5 tiles: 10.7 in
+    // two parts, 9.4 in one.  2 x 2 key heads over 50176 keys: 28.9 with two workgroups to a CU, 32.5 and 36.2 with one and four)
+    if (few && tiles >= 6) a.splits = (int)std::max<int64_t>(1, std::min<int64_t>((2 * cus + a.blocks * pairs - 1) / (a.blocks * pairs), std::min(tiles / 2, ATT_MOST_SPLITS)));
     CHIP_REQUIRE(a.blocks * pairs * a.splits < (1ll << 31), CLDNN_HIP_UNSUPPORTED_SIZE, "attention: too large");
     a.total = (int)(a.blocks * pairs * a.splits);
     const int64_t scores = (int64_t)d.batch * d.q_heads * d.q_len * d.kv_len;
@@ -400,7 +428,7 @@ void attention_launch(hipStream_t s, const AttentionPlan& p, void* workspace, co
         default: launch(std::integral_constant<int, 256>());
         }
         if (a.splits > 1)
-            hipLaunchKernelGGL((attention_join_kernel<T>), dim3(a.rows, p.a.total / a.blocks / a.splits), dim3(256), 0, s, a, (const float*)workspace, (T*)out);
+            hipLaunchKernelGGL((attention_join_kernel<T>), dim3(a.rows, p.a.total / a.blocks / a.splits), dim3(ATT_JOIN), 0, s, a, (const float*)workspace, (T*)out);
     });
     CHIP_CHECK(hipGetLastError());
 }
