@@ -15,8 +15,9 @@ struct NormArgs {
     int32_t W, P;          // width and size of the plane
     int32_t span;          // features of a workgroup: whole groups
     int32_t cols, rows;    // vectors across the features, pixels at a time
-    int32_t chunk, chunks; // pixels of a workgroup of the statistics pass; workgroups along the plane
-    int32_t chunk2;        // pixels of a workgroup of the second pass
+    int32_t fold;          // log2 of the neighbouring features that a thread's parts are of: a power of two that divides a group and a vector
+    int32_t lanes;         // threads that join the parts of a group: a power of two, up to a wave
+    int32_t chunk, chunks; // pixels of a workgroup; workgroups along the plane
     int32_t whole;         // planes without gaps between rows: pixel p lies at p * px
     float epsilon;
     Act act;
@@ -24,14 +25,12 @@ struct NormArgs {
 
 struct NormPlan {
     NormArgs a;
-    int in_dt, out_dt, vec;
-    int blocks2;
-    int spans;
-    int B;
+    int in_dt, out_dt, vec, threads, spans, B;
+    int held;  // pixels that a thread holds in registers: the whole plane in one launch; 0: two launches
 };
 
-constexpr int NORM_THREADS = 256;
 constexpr int NORM_MOST_SPAN = 6144;  // features of a workgroup: their sums lie in LDS
+constexpr int NORM_MOST_THREADS = 1024;
 
 template <typename T, int V>
 __device__ inline void norm_load(const T* p, float (&v)[V])
@@ -68,120 +67,249 @@ __device__ inline int64_t norm_pixel(const NormArgs& a, int64_t py, int64_t px, 
 // pixels of row r when n are dealt to `rows` of them in turn
 __device__ inline int norm_share(int n, int r, int rows) { return (n - r + rows - 1) / rows; }
 
-// The statistics of a workgroup's part: part[((b * chunks + chunk) * groups + g)] = (mean, M2) of group g.
-template <typename TI, int V>
-__global__ __launch_bounds__(NORM_THREADS) void norm_stats_kernel(NormArgs a, const TI* in, float2* part)
-{
-    extern __shared__ float2 lds[];
-    float2* feature = lds;              // [span] mean, M2 of each feature
-    float2* row = lds + a.span;         // [rows][cols * V] sums of each row of threads
-    const int b = blockIdx.y, first = blockIdx.z * a.span, t = threadIdx.x;
-    const int span = min(a.span, a.C - first);
-    const int p0 = blockIdx.x * a.chunk, n = min(a.chunk, a.P - p0);
-    const TI* base = in + a.in_off + b * a.in_pb + first;
-    const int r = t / a.cols;
-    for (int c0 = 0; c0 < span; c0 += a.cols * V) {
-        const int width = min(a.cols * V, span - c0), c = (t - r * a.cols) * V;
-        const bool live = r < min(a.rows, n) && c < width;
-        if (live) {
-            const TI* at = base + c0 + c;
-            float K[V], s1[V], s2[V];
-            norm_load<TI, V>(at + norm_pixel(a, a.in_py, a.in_px, p0 + r), K);
+// mean and M2 of values a vector holds
+template <int V>
+struct NormSums {
+    float K[V], s1[V], s2[V];
+    __device__ void start(const float (&v)[V])
+    {
 #pragma unroll
-            for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0f;
-#pragma unroll 4
-            for (int p = r + a.rows; p < n; p += a.rows) {
-                float v[V];
-                norm_load<TI, V>(at + norm_pixel(a, a.in_py, a.in_px, p0 + p), v);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float d = v[i] - K[i];
-                    s1[i] += d;
-                    s2[i] = __builtin_fmaf(d, d, s2[i]);
-                }
-            }
-            const float own = 1.0f / (float)norm_share(n, r, a.rows);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float m = s1[i] * own;
-                row[r * a.cols * V + c + i] = make_float2(K[i] + m, s2[i] - s1[i] * m);
-            }
-        }
-        __syncthreads();
-        for (int f = t; f < width; f += NORM_THREADS) {
-            const float K = row[f].x;
-            float mean = 0.0f, M2 = 0.0f;
-            for (int j = 0; j < min(a.rows, n); ++j) mean += (row[j * a.cols * V + f].x - K) * (float)norm_share(n, j, a.rows);
-            mean = K + mean / (float)n;
-            for (int j = 0; j < min(a.rows, n); ++j) {
-                const float2 s = row[j * a.cols * V + f];
-                const float d = s.x - mean;
-                M2 += s.y + (float)norm_share(n, j, a.rows) * d * d;
-            }
-            feature[c0 + f] = make_float2(mean, M2);
-        }
-        __syncthreads();
+        for (int i = 0; i < V; ++i) K[i] = v[i], s1[i] = s2[i] = 0.0f;
     }
-    for (int g = t; g < span / a.cpg; g += NORM_THREADS) {
-        float mean = 0.0f, M2 = 0.0f;
-        const float K = feature[g * a.cpg].x;
-        for (int i = 0; i < a.cpg; ++i) mean += feature[g * a.cpg + i].x - K;
-        mean = K + mean / (float)a.cpg;
-        for (int i = 0; i < a.cpg; ++i) {
-            const float2 f = feature[g * a.cpg + i];
-            const float d = f.x - mean;
-            M2 += f.y + (float)n * d * d;
+    __device__ void add(const float (&v)[V])
+    {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float d = v[i] - K[i];
+            s1[i] += d;
+            s2[i] = __builtin_fmaf(d, d, s2[i]);
         }
-        part[((int64_t)b * a.chunks + blockIdx.x) * a.groups + first / a.cpg + g] = make_float2(mean, M2);
+    }
+    // neighbours of one group, 2^fold of them, are one part: parts of n values each are joined two by two
+    __device__ void put(const NormArgs& a, float2* row, int c, int n) const
+    {
+        const float own = 1.0f / (float)n;
+        float mean[V], M2[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float m = s1[i] * own;
+            mean[i] = K[i] + m, M2[i] = s2[i] - s1[i] * m;
+        }
+        float half = 0.5f * (float)n;
+#pragma unroll
+        for (int step = 1; step < V; step *= 2) {
+            if (step >= 1 << a.fold) break;
+#pragma unroll
+            for (int i = 0; i < V; i += 2 * step) {
+                const float d = mean[i + step] - mean[i];
+                mean[i] = __builtin_fmaf(0.5f, d, mean[i]);
+                M2[i] = __builtin_fmaf(half * d, d, M2[i] + M2[i + step]);
+            }
+            half *= 2.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if ((i & ((1 << a.fold) - 1)) == 0) row[(c + i) >> a.fold] = make_float2(mean[i], M2[i]);
+    }
+};
+
+// Joins N parts of a group, `total` values: part(i, n) gives mean and M2 of part i and in n how many values those are of.  The a.lanes
+// threads of the group (neighbours in a wave) call this together and all get the result.  Two passes over the parts, the first
+// NORM_PARTS of a thread from registers.
+constexpr int NORM_PARTS = 8;
+template <typename P>
+__device__ inline float2 norm_join(const NormArgs& a, int N, float total, P&& part)
+{
+    const int lane = threadIdx.x & (a.lanes - 1);
+    float2 x[NORM_PARTS];
+    float n[NORM_PARTS], unused;
+    const float K = part(0, unused).x;
+#pragma unroll
+    for (int u = 0; u < NORM_PARTS; ++u) {
+        const int i = lane + u * a.lanes;
+        x[u] = make_float2(K, 0.0f), n[u] = 0.0f;
+        if (i < N) x[u] = part(i, n[u]);
+    }
+    const auto all = [&](float v) {
+        for (int i = a.lanes >> 1; i; i >>= 1) v += __shfl_xor(v, i);
+        return v;
+    };
+    float mean = 0.0f, M2 = 0.0f;
+#pragma unroll
+    for (int u = 0; u < NORM_PARTS; ++u) mean = __builtin_fmaf(x[u].x - K, n[u], mean);
+    for (int i = lane + NORM_PARTS * a.lanes; i < N; i += a.lanes) {
+        float m;
+        const float2 y = part(i, m);
+        mean = __builtin_fmaf(y.x - K, m, mean);
+    }
+    mean = K + all(mean) / total;
+#pragma unroll
+    for (int u = 0; u < NORM_PARTS; ++u) {
+        const float d = x[u].x - mean;
+        M2 += __builtin_fmaf(n[u] * d, d, x[u].y);
+    }
+    for (int i = lane + NORM_PARTS * a.lanes; i < N; i += a.lanes) {
+        float m;
+        const float2 y = part(i, m);
+        M2 += __builtin_fmaf(m * (y.x - mean), y.x - mean, y.y);
+    }
+    return make_float2(mean, all(M2));
+}
+
+// The parts that a workgroup's threads put into LDS, n pixels in all, group by group: then(g, its mean and M2).
+template <typename F>
+__device__ inline void norm_join_rows(const NormArgs& a, const float2* rows, int span, int n, F&& then)
+{
+    const int used = min(a.rows, n), base = n / a.rows, more = n - base * a.rows;  // row r has base pixels, the first `more` one more
+    const int each = a.cpg >> a.fold, pitch = a.span >> a.fold;  // parts of a group in a row, of a row
+    const float inverse = 1.0f / (float)each, values = (float)(1 << a.fold);
+    for (int g = threadIdx.x / a.lanes; g < span / a.cpg; g += blockDim.x / a.lanes) {
+        const float2 f = norm_join(a, used * each, (float)n * (float)a.cpg, [&](int i, float& m) {
+            const int r = (int)(((float)i + 0.5f) * inverse);  // i / each: there are at most 8192
+            m = (float)(base + (r < more)) * values;
+            return rows[r * pitch + g * each + i - r * each];
+        });
+        if ((threadIdx.x & (a.lanes - 1)) == 0) then(g, f);
     }
 }
 
-// The second pass: joins the parts of the workgroup's groups and writes the result for its pixels.
-template <typename TI, typename TO, int V>
-__global__ __launch_bounds__(NORM_THREADS) void norm_apply_kernel(NormArgs a, const TI* in, const float* scale, const float* shift, TO* out, const float2* part)
+__device__ inline float2 norm_scale(const NormArgs& a, float2 f)
 {
-    extern __shared__ float2 lds[];  // [groups of the span] mean, 1 / deviation
-    const int b = blockIdx.y, first = blockIdx.z * a.span, t = threadIdx.x;
-    const int span = min(a.span, a.C - first);
-    for (int g = t; g < span / a.cpg; g += NORM_THREADS) {
-        const float2* of = part + (int64_t)b * a.chunks * a.groups + first / a.cpg + g;
-        const float K = of[0].x;
-        float mean = 0.0f, M2 = 0.0f;
-        for (int k = 0; k < a.chunks; ++k) mean += (of[(int64_t)k * a.groups].x - K) * (float)min(a.chunk, a.P - k * a.chunk);
-        mean = K + mean / (float)a.P;
-        for (int k = 0; k < a.chunks; ++k) {
-            const float2 f = of[(int64_t)k * a.groups];
-            const float d = f.x - mean;
-            M2 += f.y + (float)min(a.chunk, a.P - k * a.chunk) * (float)a.cpg * d * d;
-        }
-        const float variance = M2 / ((float)a.P * (float)a.cpg);
-        lds[g] = make_float2(mean, 1.0f / __builtin_sqrtf(variance + a.epsilon));
-    }
-    __syncthreads();
-    const int p0 = blockIdx.x * a.chunk2, n = min(a.chunk2, a.P - p0), r = t / a.cols;
-    if (r >= a.rows) return;
-    const TI* src = in + a.in_off + b * a.in_pb + first;
-    TO* dst = out + a.out_off + b * a.out_pb + first;
-    for (int c = (t - r * a.cols) * V; c < span; c += a.cols * V) {
-        float mean[V], factor[V], add[V];
+    return make_float2(f.x, 1.0f / __builtin_sqrtf(f.y / ((float)a.P * (float)a.cpg) + a.epsilon));
+}
+
+// what a thread needs for its features from c on: group[g] = mean, 1 / deviation
+template <int V>
+struct NormFactors {
+    float mean[V], factor[V], add[V];
+    __device__ void get(const NormArgs& a, const float2* group, int first, int c, const float* scale, const float* shift)
+    {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const float2 f = lds[(c + i) / a.cpg];
+            const float2 f = group[(c + i) / a.cpg];
             mean[i] = f.x;
             factor[i] = scale ? f.y * scale[first + c + i] : f.y;
             add[i] = shift ? shift[first + c + i] : 0.0f;
         }
+    }
+    __device__ void use(const NormArgs& a, float (&v)[V]) const
+    {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = __builtin_fmaf(v[i] - mean[i], factor[i], add[i]);
+        act_apply(v, a.act);
+    }
+};
+
+// Groups whose plane a workgroup holds in its registers, U vectors to a thread: one read, one write, one launch.
+template <typename TI, typename TO, int V, int U>
+__global__ __launch_bounds__(NORM_MOST_THREADS) void norm_whole_kernel(NormArgs a, const TI* in, const float* scale, const float* shift, TO* out)
+{
+    typedef TI any __attribute__((ext_vector_type(V), aligned(sizeof(TI))));
+    extern __shared__ float2 lds[];
+    float2* rows = lds;                                   // parts of each row of threads
+    float2* group = lds + a.rows * (a.span >> a.fold);    // [groups of the span]
+    const int b = blockIdx.y, first = blockIdx.z * a.span, t = threadIdx.x;
+    const int span = min(a.span, a.C - first), r = t / a.cols, c = (t - r * a.cols) * V;
+    const bool live = r < min(a.rows, a.P) && c < span;
+    const TI* src = in + a.in_off + b * a.in_pb + first + c;
+    any held[U];
+    if (live) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (r + u * a.rows < a.P) held[u] = *(const any*)(src + norm_pixel(a, a.in_py, a.in_px, r + u * a.rows));
+        const auto value = [&](int u, float(&v)[V]) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = (float)held[u][i];
+        };
+        NormSums<V> sums;
+        float v[V];
+        value(0, v);
+        sums.start(v);
+#pragma unroll
+        for (int u = 1; u < U; ++u)
+            if (r + u * a.rows < a.P) value(u, v), sums.add(v);
+        sums.put(a, rows + r * (a.span >> a.fold), c, norm_share(a.P, r, a.rows));
+    }
+    __syncthreads();
+    norm_join_rows(a, rows, span, a.P, [&](int g, float2 f) { group[g] = norm_scale(a, f); });
+    __syncthreads();
+    if (!live) return;
+    NormFactors<V> factors;
+    factors.get(a, group, first, c, scale, shift);
+    TO* dst = out + a.out_off + b * a.out_pb + first + c;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (r + u * a.rows < a.P) {
+            float v[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = (float)held[u][i];
+            factors.use(a, v);
+            norm_store<TO, V>(dst + norm_pixel(a, a.out_py, a.out_px, r + u * a.rows), v);
+        }
+}
+
+// The statistics of a workgroup's pixels: part[((b * chunks + chunk) * groups + g)] = (mean, M2) of group g.
+template <typename TI, int V>
+__global__ __launch_bounds__(NORM_MOST_THREADS) void norm_stats_kernel(NormArgs a, const TI* in, float2* part)
+{
+    extern __shared__ float2 lds[];  // parts of each row of threads
+    const int b = blockIdx.y, first = blockIdx.z * a.span, t = threadIdx.x;
+    const int span = min(a.span, a.C - first);
+    const int p0 = blockIdx.x * a.chunk, n = min(a.chunk, a.P - p0), r = t / a.cols;
+    const TI* base = in + a.in_off + b * a.in_pb + first;
+    if (r < min(a.rows, n))
+        for (int c = (t - r * a.cols) * V; c < span; c += a.cols * V) {
+            NormSums<V> sums;
+            float v[V];
+            norm_load<TI, V>(base + c + norm_pixel(a, a.in_py, a.in_px, p0 + r), v);
+            sums.start(v);
+#pragma unroll 4
+            for (int p = r + a.rows; p < n; p += a.rows) {
+                norm_load<TI, V>(base + c + norm_pixel(a, a.in_py, a.in_px, p0 + p), v);
+                sums.add(v);
+            }
+            sums.put(a, lds + r * (a.span >> a.fold), c, norm_share(n, r, a.rows));
+        }
+    __syncthreads();
+    norm_join_rows(a, lds, span, n, [&](int g, float2 f) { part[((int64_t)b * a.chunks + blockIdx.x) * a.groups + first / a.cpg + g] = f; });
+}
+
+// The second pass: joins the parts of the workgroup's groups and writes the result for its pixels.
+template <typename TI, typename TO, int V>
+__global__ __launch_bounds__(NORM_MOST_THREADS) void norm_apply_kernel(NormArgs a, const TI* in, const float* scale, const float* shift, TO* out, const float2* part)
+{
+    extern __shared__ float2 lds[];  // [groups of the span] mean, 1 / deviation
+    const int b = blockIdx.y, first = blockIdx.z * a.span, t = threadIdx.x;
+    const int span = min(a.span, a.C - first);
+    const int lane = t & (a.lanes - 1);
+    for (int g = t / a.lanes; g < span / a.cpg; g += blockDim.x / a.lanes) {
+        const float2* of = part + (int64_t)b * a.chunks * a.groups + first / a.cpg + g;
+        const float2 f = norm_join(a, a.chunks, (float)a.P * (float)a.cpg, [&](int i, float& n) {
+            n = (float)min(a.chunk, a.P - i * a.chunk) * (float)a.cpg;
+            return of[(int64_t)i * a.groups];
+        });
+        if (lane == 0) lds[g] = norm_scale(a, f);
+    }
+    __syncthreads();
+    // the pixels that the first pass read last are the likeliest to be near
+    const int p0 = (a.chunks - 1 - (int)blockIdx.x) * a.chunk, n = min(a.chunk, a.P - p0), r = t / a.cols;
+    if (r >= a.rows) return;
+    const TI* src = in + a.in_off + b * a.in_pb + first;
+    TO* dst = out + a.out_off + b * a.out_pb + first;
+    for (int c = (t - r * a.cols) * V; c < span; c += a.cols * V) {
+        NormFactors<V> factors;
+        factors.get(a, lds, first, c, scale, shift);
 #pragma unroll 4
         for (int p = r; p < n; p += a.rows) {
             float v[V];
             norm_load<TI, V>(src + c + norm_pixel(a, a.in_py, a.in_px, p0 + p), v);
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = __builtin_fmaf(v[i] - mean[i], factor[i], add[i]);
-            act_apply(v, a.act);
+            factors.use(a, v);
             norm_store<TO, V>(dst + c + norm_pixel(a, a.out_py, a.out_px, p0 + p), v);
         }
     }
 }
+
+static size_t norm_lds(const NormPlan& p) { return (p.a.rows * (p.a.span >> p.a.fold) + (p.held ? p.a.span / p.a.cpg : 0)) * sizeof(float2); }
 
 NormPlan* norm_plan(const cldnn_hip_engine_s& e, const cldnn_hip_group_norm_desc& d, cldnn_hip_operator_info& info)
 {
@@ -208,27 +336,51 @@ NormPlan* norm_plan(const cldnn_hip_engine_s& e, const cldnn_hip_group_norm_desc
     int unit = a.cpg;
     while (unit % plan->vec) unit += a.cpg;
     if (unit > NORM_MOST_SPAN) unit = a.cpg, plan->vec = 1;
-    const int most = std::min(NORM_MOST_SPAN, std::max(unit, NORM_THREADS * plan->vec / unit * unit));
-    a.span = std::min(a.C, most / unit * unit);
-    plan->spans = (a.C + a.span - 1) / a.span;
-    CHIP_REQUIRE(plan->spans <= 65535, CLDNN_HIP_UNSUPPORTED_SIZE, "group norm: too many features");
-    a.cols = std::min(a.span / plan->vec, NORM_THREADS);
-    a.rows = NORM_THREADS / a.cols;
-    const int cus = e.props.multiProcessorCount;
-    const int64_t wanted = std::max<int64_t>(1, (int64_t)cus * 4 / ((int64_t)it.b * plan->spans));
-    a.chunk = (int)std::max<int64_t>((a.P + wanted - 1) / wanted, std::min(a.P, a.rows * 4));
+    const int V = plan->vec, cus = e.props.multiProcessorCount;
+    while (2 << a.fold <= V && a.cpg % (2 << a.fold) == 0) ++a.fold;
+    const auto shape = [&](int span, int threads) {
+        a.span = std::min(a.C, span);
+        plan->threads = threads;
+        plan->spans = (a.C + a.span - 1) / a.span;
+        a.cols = std::min((a.span + V - 1) / V, threads);
+        a.rows = threads / a.cols;
+        const int in_span = a.span / a.cpg;
+        a.lanes = 64;
+        while (a.lanes > 1 && a.lanes * in_span > threads) a.lanes >>= 1;
+    };
+    // In registers: the fewest groups that make runs of 64 bytes, as many threads as hold their plane in up to 16 vectors of 16 bytes.
+    const int most = is == 4 ? 8 : 16;
+    int span = unit;
+    while (span * is < 64 && span < a.C) span += unit;
+    span = std::min(span, a.C);
+    plan->held = 0;
+    if (span <= NORM_MOST_THREADS * V)
+        for (int threads = 256; threads <= NORM_MOST_THREADS && !plan->held; threads *= 2) {
+            const int rows = threads / ((span + V - 1) / V);
+            if (rows < 1) continue;
+            const int held = (a.P + rows - 1) / rows;
+            if (held <= (threads < NORM_MOST_THREADS ? 4 : most)) {
+                shape(span, threads);
+                for (plan->held = 1; plan->held < held;) plan->held *= 2;
+            }
+        }
+    if (!plan->held) {
+        shape(std::max(unit, std::min(NORM_MOST_SPAN, NORM_MOST_THREADS * V) / unit * unit), NORM_MOST_THREADS);
+        const int64_t wanted = std::max<int64_t>(1, (int64_t)cus / ((int64_t)it.b * plan->spans));
+        a.chunk = (int)std::max<int64_t>((a.P + wanted - 1) / wanted, std::min(a.P, a.rows * 2));
+    } else a.chunk = a.P;
     a.chunks = (a.P + a.chunk - 1) / a.chunk;
-    a.chunk2 = (int)std::max<int64_t>((a.P + 2 * wanted - 1) / (2 * wanted), std::min(a.P, a.rows * 4));
-    plan->blocks2 = (a.P + a.chunk2 - 1) / a.chunk2;
+    CHIP_REQUIRE(plan->spans <= 65535, CLDNN_HIP_UNSUPPORTED_SIZE, "group norm: too many features");
     plan->in_dt = it.dtype, plan->out_dt = ot.dtype, plan->B = it.b;
     const int64_t n = (int64_t)it.b * a.P * a.C;
-    info.launches = 2;
-    info.grid = a.chunks * it.b * plan->spans, info.block = NORM_THREADS;
-    info.lds_bytes = (int)((a.span + a.rows * a.cols * plan->vec) * sizeof(float2));
-    info.workspace_bytes = (int64_t)it.b * a.chunks * a.groups * (int64_t)sizeof(float2);
+    info.launches = plan->held ? 1 : 2;
+    info.grid = a.chunks * it.b * plan->spans, info.block = plan->threads;
+    info.lds_bytes = (int)norm_lds(*plan);
+    if (!plan->held) info.workspace_bytes = (int64_t)it.b * a.chunks * a.groups * (int64_t)sizeof(float2);
     info.ops = 10 * n;
     info.bytes = n * (is + os) + 8 * (int64_t)a.C;
-    snprintf(info.kernel_name, sizeof info.kernel_name, "norm_stats<v%d> + norm_apply<v%d>", plan->vec, plan->vec);
+    if (plan->held) snprintf(info.kernel_name, sizeof info.kernel_name, "norm_whole<v%d,%d>", V, plan->held);
+    else snprintf(info.kernel_name, sizeof info.kernel_name, "norm_stats<v%d> + norm_apply<v%d>", V, V);
     return plan.release();
 }
 
@@ -242,10 +394,23 @@ void norm_launch(hipStream_t s, const NormPlan& p, void* workspace, const void* 
         typedef decltype(ti) TI;
         typedef decltype(to) TO;
         constexpr int V = decltype(v)::value;
-        const size_t lds = (a.span + a.rows * a.cols * V) * sizeof(float2);
-        hipLaunchKernelGGL((norm_stats_kernel<TI, V>), dim3(a.chunks, p.B, p.spans), dim3(NORM_THREADS), lds, s, a, (const TI*)in, part);
-        hipLaunchKernelGGL((norm_apply_kernel<TI, TO, V>), dim3(p.blocks2, p.B, p.spans), dim3(NORM_THREADS), a.span / a.cpg * sizeof(float2), s, a,
-                           (const TI*)in, scale, shift, (TO*)out, part);
+        const dim3 grid(a.chunks, p.B, p.spans), block(p.threads);
+        const auto whole = [&](auto u) {
+            constexpr int U = decltype(u)::value;
+            hipLaunchKernelGGL((norm_whole_kernel<TI, TO, V, U>), grid, block, norm_lds(p), s, a, (const TI*)in, scale, shift, (TO*)out);
+        };
+        switch (p.held) {
+        case 0:
+            hipLaunchKernelGGL((norm_stats_kernel<TI, V>), grid, block, norm_lds(p), s, a, (const TI*)in, part);
+            hipLaunchKernelGGL((norm_apply_kernel<TI, TO, V>), grid, block, a.span / a.cpg * sizeof(float2), s, a, (const TI*)in, scale, shift, (TO*)out, part);
+            break;
+        case 1: whole(std::integral_constant<int, 1>()); break;
+        case 2: whole(std::integral_constant<int, 2>()); break;
+        case 4: whole(std::integral_constant<int, 4>()); break;
+        case 8: whole(std::integral_constant<int, 8>()); break;
+        default:
+            if constexpr (sizeof(TI) == 2) whole(std::integral_constant<int, 16>());
+        }
     };
     with_float(p.in_dt, [&](auto ti) {
         with_float(p.out_dt, [&](auto to) {
