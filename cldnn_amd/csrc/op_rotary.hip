@@ -19,14 +19,16 @@ struct RotaryPair {
 struct RotaryArgs {
     int64_t tokens;
     int32_t q_heads, k_heads, pairs, axes, copied;  // values behind the pairs, copied
-    int32_t head_size;
+    int32_t items;      // threads of a token and its group of heads: W pairs each, then 8 of the copied values each
+    int32_t heads;      // of a group
+    int32_t interleaved;
     int32_t float_positions, inverse;
     int64_t q_pt, q_ph, k_pt, k_ph, qo_pt, qo_ph, ko_pt, ko_ph;
 };
 
 struct RotaryPlan {
     RotaryArgs a;
-    int dt, pos_size, work;
+    int dt, width, groups;
 };
 
 constexpr int ROTARY_THREADS = 256;
@@ -40,41 +42,75 @@ __device__ inline void rotary_turn(float position, const RotaryPair& p, float& s
     sincospif(2.0f * turns, &s, &c);
 }
 
-// A thread turns one pair (or copies one value) of a token in all of its heads: one sine and cosine for all of them.
-template <typename T>
+template <typename T, int N>
+struct RotaryVector {
+    typedef T any __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    any v;
+    __device__ void load(const T* p) { v = *(const any*)p; }
+    __device__ void store(T* p) const { *(any*)p = v; }
+};
+
+// A thread turns W neighbouring pairs of a token in a group of its heads, queries' first, keys' behind them: one sine and cosine
+// for all of them, worked out while the first heads' values are on their way.  Their values are two runs of W, or where pairs are
+// interleaved one of 2 W.
+template <typename T, int W, bool INTERLEAVED>
 __global__ __launch_bounds__(ROTARY_THREADS) void rotary_kernel(RotaryArgs a, const RotaryPair* table, const void* positions, const T* q, const T* k, T* qo, T* ko)
 {
-    const int work = a.pairs + a.copied;
+    constexpr int AT_ONCE = 4;
     const int64_t i = (int64_t)blockIdx.x * ROTARY_THREADS + threadIdx.x;
-    const int64_t token = i / work;
-    const int w = (int)(i - token * work);
+    const int64_t token = i / a.items;
+    const int w = (int)(i - token * a.items);
     if (token >= a.tokens) return;
-    q += token * a.q_pt, qo += token * a.qo_pt;
-    if (a.k_heads) k += token * a.k_pt, ko += token * a.ko_pt;
-    if (w >= a.pairs) {
-        const int at = a.pairs + w;
-        for (int h = 0; h < a.q_heads; ++h) qo[h * a.qo_ph + at] = q[h * a.q_ph + at];
-        for (int h = 0; h < a.k_heads; ++h) ko[h * a.ko_ph + at] = k[h * a.k_ph + at];
+    const int from = blockIdx.y * a.heads, to = min(from + a.heads, a.q_heads + a.k_heads);
+    const auto source = [&](int h) { return h < a.q_heads ? q + token * a.q_pt + h * a.q_ph : k + token * a.k_pt + (h - a.q_heads) * a.k_ph; };
+    const auto target = [&](int h) { return h < a.q_heads ? qo + token * a.qo_pt + h * a.qo_ph : ko + token * a.ko_pt + (h - a.q_heads) * a.ko_ph; };
+    if (w * W >= a.pairs) {
+        const int at = 2 * a.pairs + (w - a.pairs / W) * 8, n = min(8, 2 * a.pairs + a.copied - at);
+        for (int h = from; h < to; ++h)
+            for (int j = 0; j < n; ++j) target(h)[at + j] = source(h)[at + j];
         return;
     }
-    const RotaryPair p = table[w];
-    const int64_t at = token * a.axes + p.axis;
-    float s, c;
-    rotary_turn(a.float_positions ? ((const float*)positions)[at] : (float)((const int32_t*)positions)[at], p, s, c);
-    if (a.inverse) s = -s;
-    const auto turn = [&](const T* x, T* y, int heads, int64_t xp, int64_t yp) {
-#pragma unroll 4
-        for (int h = 0; h < heads; ++h) {
-            const float x0 = (float)x[h * xp + p.first], x1 = (float)x[h * xp + p.second];
-            y[h * yp + p.first] = (T)(x0 * c - x1 * s);
-            y[h * yp + p.second] = (T)(x1 * c + x0 * s);
-        }
-    };
-    turn(q, qo, a.q_heads, a.q_ph, a.qo_ph);
-    turn(k, ko, a.k_heads, a.k_ph, a.ko_ph);
+    typedef RotaryVector<T, INTERLEAVED ? 2 * W : W> Run;
+    RotaryPair p[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) p[j] = table[w * W + j];
+    float s[W], c[W], position[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        const int64_t at = token * a.axes + p[j].axis;
+        position[j] = a.float_positions ? ((const float*)positions)[at] : (float)((const int32_t*)positions)[at];
+    }
+    for (int h = from; h < to; h += AT_ONCE) {
+        Run x[AT_ONCE], y[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+            if (h + u < to) {
+                x[u].load(source(h + u) + p[0].first);
+                if constexpr (!INTERLEAVED) y[u].load(source(h + u) + p[0].second);
+            }
+        if (h == from)
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                rotary_turn(position[j], p[j], s[j], c[j]);
+                if (a.inverse) s[j] = -s[j];
+            }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+            if (h + u < to) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    const float x0 = (float)x[u].v[INTERLEAVED ? 2 * j : j], x1 = (float)(INTERLEAVED ? x[u].v[(2 * j + 1) % (2 * W)] : y[u].v[j]);
+                    const T y0 = (T)(x0 * c[j] - x1 * s[j]), y1 = (T)(x1 * c[j] + x0 * s[j]);
+                    if constexpr (INTERLEAVED) x[u].v[2 * j] = y0, x[u].v[2 * j + 1] = y1;
+                    else x[u].v[j] = y0, y[u].v[j] = y1;
+                }
+                x[u].store(target(h + u) + p[0].first);
+                if constexpr (!INTERLEAVED) y[u].store(target(h + u) + p[0].second);
+            }
+    }
 }
 
-RotaryPlan* rotary_plan(const cldnn_hip_engine_s&, const cldnn_hip_rotary_desc& d, cldnn_hip_operator_info& info, std::vector<char>& init)
+RotaryPlan* rotary_plan(const cldnn_hip_engine_s& e, const cldnn_hip_rotary_desc& d, cldnn_hip_operator_info& info, std::vector<char>& init)
 {
     const int size = float_size(d.dtype, "rotary");
     CHIP_REQUIRE(d.tokens > 0 && d.q_heads > 0 && d.k_heads >= 0 && d.head_size > 0, CLDNN_HIP_INVALID_ARG, "rotary: sizes must be positive");
@@ -90,7 +126,7 @@ RotaryPlan* rotary_plan(const cldnn_hip_engine_s&, const cldnn_hip_rotary_desc& 
     CHIP_REQUIRE(pairs > 0 && 2 * pairs <= d.head_size, CLDNN_HIP_DIMENSION_MISMATCH, "rotary: the axes' pairs must be some, and fit the head");
     std::unique_ptr<RotaryPlan> plan(new RotaryPlan{});
     RotaryArgs& a = plan->a;
-    a.tokens = d.tokens, a.q_heads = d.q_heads, a.k_heads = d.k_heads, a.axes = d.axes, a.head_size = d.head_size;
+    a.tokens = d.tokens, a.q_heads = d.q_heads, a.k_heads = d.k_heads, a.axes = d.axes, a.interleaved = d.pairing == CLDNN_HIP_ROTARY_INTERLEAVED;
     a.pairs = (int)pairs, a.copied = d.head_size - 2 * (int)pairs;
     a.float_positions = d.position_dtype == CLDNN_HIP_F32, a.inverse = d.inverse != 0;
     const auto strides = [&](int heads, int64_t token, int64_t head, int64_t& pt, int64_t& ph) {
@@ -118,14 +154,30 @@ RotaryPlan* rotary_plan(const cldnn_hip_engine_s&, const cldnn_hip_rotary_desc& 
         }
         start += d.pairs[axis];
     }
-    plan->dt = d.dtype, plan->work = a.pairs + a.copied;
-    const int64_t blocks = (d.tokens * plan->work + ROTARY_THREADS - 1) / ROTARY_THREADS;
+    plan->dt = d.dtype;
+    // 16 bytes to a run where the pairs can be taken so, by halves of it otherwise; a run stays within an axis where that sets its place
+    plan->width = 16 / size / (a.interleaved ? 2 : 1);
+    const auto fits = [&](int w) {
+        if (d.pairing == CLDNN_HIP_ROTARY_HALVES_PER_AXIS)
+            for (int i = 0; i < d.axes; ++i)
+                if (d.pairs[i] % w) return false;
+        return pairs % w == 0;
+    };
+    while (!fits(plan->width)) plan->width /= 2;
+    a.items = a.pairs / plan->width + (a.copied + 7) / 8;
+    const int64_t blocks = (d.tokens * a.items + ROTARY_THREADS - 1) / ROTARY_THREADS;
     CHIP_REQUIRE(d.tokens < (1ll << 40) && blocks < (1ll << 31), CLDNN_HIP_UNSUPPORTED_SIZE, "rotary: too many tokens");
+    // heads in groups where threads are few: four waves to a SIMD before a thread takes a second group of four
+    const int heads = d.q_heads + d.k_heads;
+    const int64_t wanted = std::max<int64_t>(1, 4ll * e.props.multiProcessorCount / blocks);
+    a.heads = (int)((heads + wanted - 1) / wanted);
+    plan->groups = (heads + a.heads - 1) / a.heads;
+    CHIP_REQUIRE(plan->groups <= 65535, CLDNN_HIP_UNSUPPORTED_SIZE, "rotary: too many heads");
     const int64_t n = d.tokens * (d.q_heads + d.k_heads) * d.head_size;
-    info.launches = 1, info.grid = (int)blocks, info.block = ROTARY_THREADS;
+    info.launches = 1, info.grid = (int)blocks * plan->groups, info.block = ROTARY_THREADS;
     info.workspace_bytes = (int64_t)init.size();
     info.ops = 3 * n, info.bytes = 2 * n * size + 4 * d.tokens * d.axes;
-    snprintf(info.kernel_name, sizeof info.kernel_name, "rotary");
+    snprintf(info.kernel_name, sizeof info.kernel_name, "rotary<%d%s>", plan->width, a.interleaved ? ",interleaved" : "");
     return plan.release();
 }
 
@@ -136,11 +188,20 @@ void rotary_launch(hipStream_t s, const RotaryPlan& p, const void* workspace, co
     const int size = float_size(p.dt, "");
     check_aligned(q, size, "q"), check_aligned(k, size, "k"), check_aligned(positions, 4, "positions");
     check_aligned(q_out, size, "q output"), check_aligned(k_out, size, "k output");
-    const dim3 grid((unsigned)((a.tokens * p.work + ROTARY_THREADS - 1) / ROTARY_THREADS));
+    const dim3 grid((unsigned)((a.tokens * a.items + ROTARY_THREADS - 1) / ROTARY_THREADS), p.groups);
     with_float(p.dt, [&](auto t) {
         typedef decltype(t) T;
-        hipLaunchKernelGGL((rotary_kernel<T>), grid, dim3(ROTARY_THREADS), 0, s, a, (const RotaryPair*)workspace, positions, (const T*)q, (const T*)k,
-                           (T*)q_out, (T*)k_out);
+        const auto launch = [&](auto w) {
+            constexpr int W = decltype(w)::value;
+            const auto f = a.interleaved ? rotary_kernel<T, W <= 4 ? W : 1, true> : rotary_kernel<T, W, false>;
+            hipLaunchKernelGGL(f, grid, dim3(ROTARY_THREADS), 0, s, a, (const RotaryPair*)workspace, positions, (const T*)q, (const T*)k, (T*)q_out, (T*)k_out);
+        };
+        switch (p.width) {
+        case 8: launch(std::integral_constant<int, 8>()); break;
+        case 4: launch(std::integral_constant<int, 4>()); break;
+        case 2: launch(std::integral_constant<int, 2>()); break;
+        default: launch(std::integral_constant<int, 1>());
+        }
     });
     CHIP_CHECK(hipGetLastError());
 }

@@ -87,24 +87,29 @@ __device__ inline float act_one(float v, float m, float n)
     return v;
 }
 
-// N values with one activation: one uniform branch for all of them
+// f(the activation as a constant): one uniform branch around whatever f does with it
+template <typename F>
+__device__ inline void act_choose(int kind, F&& f)
+{
+    switch (kind) {
+    case CLDNN_HIP_ACT_RELU: return f(std::integral_constant<int, CLDNN_HIP_ACT_RELU>());
+    case CLDNN_HIP_ACT_RELU_SLOPE: return f(std::integral_constant<int, CLDNN_HIP_ACT_RELU_SLOPE>());
+    case CLDNN_HIP_ACT_CLAMP: return f(std::integral_constant<int, CLDNN_HIP_ACT_CLAMP>());
+    case CLDNN_HIP_ACT_SILU: return f(std::integral_constant<int, CLDNN_HIP_ACT_SILU>());
+    case CLDNN_HIP_ACT_GELU: return f(std::integral_constant<int, CLDNN_HIP_ACT_GELU>());
+    case CLDNN_HIP_ACT_GELU_TANH: return f(std::integral_constant<int, CLDNN_HIP_ACT_GELU_TANH>());
+    default: return f(std::integral_constant<int, CLDNN_HIP_ACT_NONE>());
+    }
+}
+
+// N values with one activation
 template <int N>
 __device__ inline void act_apply(float (&v)[N], const Act& a)
 {
-#define CHIP_ACT_CASE(K)                                               \
-    case K:                                                            \
-        _Pragma("unroll") for (int i = 0; i < N; ++i) v[i] = act_one<K>(v[i], a.m, a.n); \
-        break
-    switch (a.kind) {
-        CHIP_ACT_CASE(CLDNN_HIP_ACT_RELU);
-        CHIP_ACT_CASE(CLDNN_HIP_ACT_RELU_SLOPE);
-        CHIP_ACT_CASE(CLDNN_HIP_ACT_CLAMP);
-        CHIP_ACT_CASE(CLDNN_HIP_ACT_SILU);
-        CHIP_ACT_CASE(CLDNN_HIP_ACT_GELU);
-        CHIP_ACT_CASE(CLDNN_HIP_ACT_GELU_TANH);
-    default: break;
-    }
-#undef CHIP_ACT_CASE
+    act_choose(a.kind, [&](auto kind) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = act_one<decltype(kind)::value>(v[i], a.m, a.n);
+    });
 }
 
 // ----------------------------------------------------------------------------- operator objects
