@@ -8,12 +8,14 @@ has to be ordered by the caller (Engine.finish, events).
 import ctypes as C
 import os
 
+import numpy as np
+
 from . import hip
 
 LIB_PATH = os.path.join(os.path.dirname(hip.LIB_PATH), "libcldnn_hip_ops.so")
 
 F32, F16, BF16, I32, NO_TYPE = hip.F32, 4, 5, hip.I32, hip.NO_TYPE
-DT_NAME = {"f32": F32, "f16": F16, "bf16": BF16}
+DT_NAME = {"f32": F32, "f16": F16, "bf16": BF16, "i32": I32}
 POSITION_NAME = {"i32": I32, "f32": F32}
 ACT_NAME = dict(hip.ACT_NAME, silu=4, gelu=5, gelu_tanh=6)
 PAIRING_NAME = {"interleaved": 0, "halves": 1, "halves_per_axis": 2}
@@ -100,6 +102,58 @@ def _type(dt):
 
 def _act(act):
     return ACT_NAME[act] if isinstance(act, str) else act
+
+
+class Buffer:
+    """Device memory for a tensor of the operators' types, zeros at first (a hip.Buffer knows the convolution path's types only)."""
+
+    def __init__(self, engine, nbytes):
+        self.engine, self.nbytes, self.h = engine, nbytes, None
+        h = _P()
+        hip.check(hip.lib().cldnn_hip_buffer_alloc(engine.h, nbytes, C.byref(h)))
+        self.h = h
+
+    @property
+    def ptr(self):
+        return hip.lib().cldnn_hip_buffer_device_ptr(self.h)
+
+    def write(self, values, dtype):
+        """numpy values, rounded to `dtype`; behind what the engine has been given so far"""
+        a = to_type(values, dtype)
+        assert a.nbytes <= self.nbytes, (a.nbytes, self.nbytes)
+        hip.check(hip.lib().cldnn_hip_buffer_write(self.h, 0, a.ctypes.data, a.nbytes))
+        return self
+
+    def read(self, shape, dtype):
+        """the first values as numpy float32 (i32: int32); waits for the engine"""
+        n = {F32: np.float32, I32: np.int32, F16: np.float16, BF16: np.uint16}[_type(dtype)]
+        a = np.empty(shape, n)
+        assert a.nbytes <= self.nbytes, (a.nbytes, self.nbytes)
+        hip.check(hip.lib().cldnn_hip_buffer_read(self.h, 0, a.ctypes.data, a.nbytes))
+        if _type(dtype) == BF16:
+            return (a.astype(np.uint32) << 16).view(np.float32)
+        return a if _type(dtype) == I32 else a.astype(np.float32)
+
+    def close(self):
+        if self.h:
+            hip.check(hip.lib().cldnn_hip_buffer_release(self.h))
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def to_type(values, dtype):
+    """numpy array of the bits of `values` in an operator's type; bf16, which numpy has not, as uint16 rounded to nearest even"""
+    dt = _type(dtype)
+    if dt == BF16:
+        bits = np.ascontiguousarray(values, np.float32).view(np.uint32)
+        rounded = ((bits + 0x7fff + ((bits >> 16) & 1)) >> 16).astype(np.uint16)
+        return np.where(np.isnan(values), np.uint16(0x7fc0), rounded)
+    return np.ascontiguousarray(values, {F32: np.float32, F16: np.float16, I32: np.int32}[dt])
 
 
 class Operator:
