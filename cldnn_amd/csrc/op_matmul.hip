@@ -45,7 +45,7 @@ __device__ inline v4i matmul_load8(const T* row, int k, int K)
 }
 
 template <typename R, int N>
-__device__ inline void matmul_read(const R* p, int valid, float (&v)[N])
+__device__ __forceinline__ void matmul_read(const R* p, int valid, float (&v)[N])
 {
     if (valid >= N) {
         constexpr int W = 16 / sizeof(R) < N ? 16 / sizeof(R) : N;
@@ -63,7 +63,7 @@ __device__ inline void matmul_read(const R* p, int valid, float (&v)[N])
 }
 
 template <typename O, int N>
-__device__ inline void matmul_write(O* p, int valid, const float (&v)[N])
+__device__ __forceinline__ void matmul_write(O* p, int valid, const float (&v)[N])
 {
     if (valid >= N) {
         constexpr int W = 16 / sizeof(O) < N ? 16 / sizeof(O) : N;
@@ -82,13 +82,12 @@ __device__ inline void matmul_write(O* p, int valid, const float (&v)[N])
     }
 }
 
-// N neighbouring features from n0 on of row m, with their bias: the activations, the residual, the result
+// N neighbouring features from n0 on of row m behind their activation: the residual, the result
 template <typename T, int N>
-__device__ inline void matmul_finish(const MatmulArgs& a, float (&v)[N], int m, int n0, void* out)
+__device__ __forceinline__ void matmul_write_row(const MatmulArgs& a, float (&v)[N], int m, int n0, void* out)
 {
     const int valid = a.n - n0;
     if (m >= a.m || valid <= 0) return;
-    act_apply(v, a.act);
     if (a.residual) {
         float r[N];
         const int64_t at = m * a.r_pitch + n0;
@@ -201,7 +200,8 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_split_kernel(MatmulArgs a, 
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] += b[i];
         }
-        matmul_finish<T>(a, v, m0 + row, n, out);
+        act_apply(v, a.act);
+        matmul_write_row<T>(a, v, m0 + row, n, out);
     }
 }
 
@@ -339,18 +339,23 @@ __global__ __launch_bounds__(64 * WM * WN * KG, KG > 2 ? KG : 2) void matmul_til
             if (a.bias && n < a.n) matmul_read(a.bias + n, a.n - n, bias);
 #pragma unroll
             for (int l = 0; l < 16; ++l) v[l] += bias[l];
-            matmul_finish<T>(a, v, m0 + (wm * MB + i) * 16 + r, n, out);
+            act_apply(v, a.act);
+            matmul_write_row<T>(a, v, m0 + (wm * MB + i) * 16 + r, n, out);
         }
-        return;
-    }
-    float bias[16] = {};
-    if (a.bias && n < a.n) matmul_read(a.bias + n, a.n - n, bias);
+    } else {
+        float bias[16] = {};
+        if (a.bias && n < a.n) matmul_read(a.bias + n, a.n - n, bias);
+        act_choose(a.act.kind, [&](auto kind) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < MB; ++i) {
-        float v[16];
+            for (int i = 0; i < MB; ++i) {
+                float v[16];
 #pragma unroll
-        for (int l = 0; l < 16; ++l) v[l] = acc[l / 4][i][l % 4] + bias[l];
-        matmul_finish<T>(a, v, m0 + (wm * MB + i) * 16 + r, n, out);
+                for (int l = 0; l < 16; ++l) v[l] = acc[l / 4][i][l % 4] + bias[l];
+#pragma unroll
+                for (int l = 0; l < 16; ++l) v[l] = act_one<decltype(kind)::value>(v[l], a.act.m, a.act.n);
+                matmul_write_row<T>(a, v, m0 + (wm * MB + i) * 16 + r, n, out);
+            }
+        });
     }
 }
 

@@ -235,7 +235,7 @@ __device__ inline void norm_finish(const NormArgs& a, const TI* src, TO* dst, in
     if (live) ask(c0);
     ready();
     if (!live) return;
-    const auto finish = [&](auto kind) {
+    const auto finish = [&](auto kind) __attribute__((always_inline)) {
         for (int c = c0; c < span; c += a.cols * V) {
             if (c != c0) ask(c);
 #pragma unroll

@@ -89,7 +89,7 @@ __device__ inline float act_one(float v, float m, float n)
 
 // f(the activation as a constant): one uniform branch around whatever f does with it
 template <typename F>
-__device__ inline void act_choose(int kind, F&& f)
+__device__ __forceinline__ void act_choose(int kind, F&& f)
 {
     switch (kind) {
     case CLDNN_HIP_ACT_RELU: return f(std::integral_constant<int, CLDNN_HIP_ACT_RELU>());
@@ -106,7 +106,7 @@ __device__ inline void act_choose(int kind, F&& f)
 template <int N>
 __device__ inline void act_apply(float (&v)[N], const Act& a)
 {
-    act_choose(a.kind, [&](auto kind) {
+    act_choose(a.kind, [&](auto kind) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = act_one<decltype(kind)::value>(v[i], a.m, a.n);
     });
