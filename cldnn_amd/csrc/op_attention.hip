@@ -386,7 +386,8 @@ AttentionPlan* attention_plan(const cldnn_hip_engine_s& e, const cldnn_hip_atten
     info.ops = 4 * scores * d.head_size;
     info.bytes = 4ll * d.batch * d.head_size * ((int64_t)d.q_len * d.q_heads + (int64_t)d.kv_len * d.kv_heads)
                  + bias_size * (a.b_pb ? d.batch : 1) * (a.b_ph ? d.q_heads : 1) * (a.b_pq ? d.q_len : 1) * (int64_t)d.kv_len;
-    snprintf(info.kernel_name, sizeof info.kernel_name, "attention<%d%s%s>", plan->size, plan->waves == 1 ? ",one wave" : "", a.splits > 1 ? ",split keys" : "");
+    snprintf(info.kernel_name, sizeof info.kernel_name, "attention<%d,%d wave%s%s%s>", plan->size, plan->waves, plan->waves > 1 ? "s" : "",
+             plan->far ? ",far" : "", a.splits > 1 ? ",split keys" : "");
     return plan.release();
 }
 

@@ -377,7 +377,7 @@ enum { MM_256, MM_224, MM_192, MM_128, MM_64x128, MM_64, MM_32, MM_ANY_64, MM_AN
 static const MatmulKernel matmul_kernels[] = {
     {"matmul_tile<256x256>", 256, 256, 8}, {"matmul_tile<224x256>", 224, 256, 8}, {"matmul_tile<192x256>", 192, 256, 8},
     {"matmul_tile<128x128>", 128, 128, 4}, {"matmul_tile<64x128>", 64, 128, 4}, {"matmul_tile<64x64,k2>", 64, 64, 8}, {"matmul_tile<32x64,k4>", 32, 64, 8},
-    {"matmul_split<64x64>", 64, 64, 4}, {"matmul_split<32x32>", 32, 32, 8}, {"matmul_split<16x16>", 16, 16, 16},
+    {"matmul_split<64x64>", 64, 64, 4}, {"matmul_split<32x32>", 32, 32, 8}, {"matmul_split<16x16>", 16, 16, 8},
 };
 
 static int64_t matmul_count(int m, int n, const MatmulKernel& k) { return (int64_t)((m + k.rows - 1) / k.rows) * ((n + k.features - 1) / k.features); }
@@ -387,7 +387,7 @@ static int matmul_choose(int m, int n, bool whole, int cus)
 {
     const auto tiles = [&](int row) { return matmul_count(m, n, matmul_kernels[row]); };
     const auto rounds = [&](int row) { return (tiles(row) + cus - 1) / cus; };
-    // Few tiles of any size: the smallest, whose 16 waves split K.  (us, against 32 x 64 tiles: 1 x 2048 -> 1000 4.7 and 7.0, 64 x 2048
+    // Few tiles of any size: the smallest, whose eight waves split K.  (us, against 32 x 64 tiles: 1 x 2048 -> 1000 4.7 and 7.0, 64 x 2048
     // -> 1000 6.0 and 7.0; at twice as many tiles, 32 x 1024 -> 4096, 6.0 and 5.2)
     if (tiles(MM_16) * 4 <= cus * 5) return MM_16;
     if (!whole) return tiles(MM_ANY_64) >= cus ? MM_ANY_64 : MM_ANY_32;
@@ -489,7 +489,7 @@ void matmul_launch(hipStream_t s, const MatmulPlan& p, void* workspace, const vo
         case MM_32: launch(matmul_tile_kernel<T, 2, 1, 1, 3, 4>); break;
         case MM_ANY_64: launch(matmul_split_kernel<T, 4, 4, 2, 4>); break;
         case MM_ANY_32: launch(matmul_split_kernel<T, 2, 2, 4, 8>); break;
-        default: launch(matmul_split_kernel<T, 1, 1, 8, 16>);
+        default: launch(matmul_split_kernel<T, 1, 1, 16, 8>);
         }
     });
     CHIP_CHECK(hipGetLastError());

@@ -175,6 +175,33 @@ def test_nan_and_infinity_within_the_lengths_count(eng, lq):
     assert torch.equal(bad, want)
 
 
+@pytest.mark.parametrize("size,head,kernel", [
+    ((6, 512, 100, 16, 16), 64, "<64,8 waves>"), ((6, 512, 70, 16, 8), 128, "<128,8 waves>"), ((4, 1030, 130, 4, 4), 104, "<128,4 waves>"), ((6, 512, 70, 16, 16), 120, "<128,8 waves>"), ((4, 1030, 130, 4, 4), 32, "<32,4 waves>"),
+    ((2, 1030, 65, 8, 8), 160, "<160,4 waves>"), ((1, 30, 1000, 2, 2), 200, "<256,4 waves,split keys>"), ((1, 30, 1000, 2, 2), 96, "<96,1 wave,split keys>"), ((1, 1, 200, 2, 2), 64, "<64,1 wave>")], ids=str)
+def test_every_kernel(eng, size, head, kernel):
+    b, lq, lk, h, kv = size
+    op = ops.Attention(eng, ops.attention_desc(b, lq, lk, h, kv, head, "bf16", key_lengths=True))
+    assert op.info().kernel_name.decode() == "attention" + kernel
+    op.close()
+    check(eng, *size, head, "bf16", lengths=[lk - 7 * i for i in range(b)])
+
+
+def test_keys_too_far_apart_for_32_bits_within_a_tile(eng):
+    # 2^24 elements from key to key, as many rows as share tiles between four waves
+    lq, lk, d, pitch = 16400, 70, 32, 1 << 24
+    g = generator(19)
+    q, k, v = (random(g, 1, n, 1, d, dtype="bf16") for n in (lq, lk, lk))
+    far = torch.empty(2, (lk - 1) * pitch + 64, dtype=torch.bfloat16, device="cuda")
+    for i in range(lk):
+        far[0, i * pitch:i * pitch + d], far[1, i * pitch:i * pitch + d] = k[0, i, 0].cuda(), v[0, i, 0].cuda()
+    out = torch.empty(1, lq, 1, d, dtype=torch.bfloat16, device="cuda")
+    op = ops.Attention(eng, ops.attention_desc(1, lq, lk, 1, 1, d, "bf16", k_strides=(0, pitch, d), v_strides=(0, pitch, d)))
+    assert "4 waves,far" in op.info().kernel_name.decode()
+    run(eng, op, q.cuda(), far[0], far[1], out)
+    op.close()
+    close(out, *reference(q, k, v, d ** -0.5, None, None, "bf16"))
+
+
 @pytest.mark.parametrize("lq", [2, 40])
 def test_offsets_past_32_bits(eng, lq):
     # tokens 2^30 elements apart: the last of 5 starts 8 GiB in

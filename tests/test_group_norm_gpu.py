@@ -119,6 +119,26 @@ def test_in_place(eng, size):
     op.close()
 
 
+def test_maps_larger_than_the_caches(eng):
+    g = generator(21)
+    check(eng, torch.randn((8, 201, 200, 128), generator=g) * 2 + 1, 32, "f16", "f16", "silu", scale=random(g, 128))
+
+
+def test_offsets_past_32_bits(eng):
+    # 2^26 elements from pixel to pixel: the last starts 10 GiB in
+    y, x, f, spare = 9, 9, 24, (1 << 26) - 24
+    g = generator(23)
+    data = random(g, 1, y, x, f, dtype="bf16")
+    src, dst = (torch.empty(y * x << 26, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    src.view(y * x, 1 << 26)[:, :f] = data.view(y * x, f).cuda()
+    t = ops.map_tensor("bf16", 1, y, x, f, pad_f=spare)
+    op = ops.GroupNorm(eng, ops.group_norm_desc(t, 3, output=t))
+    run(eng, op, src, dst)
+    op.close()
+    _, want, bound = reference(data, 3, None, None, 1e-5, "none", 0, 0)
+    close(dst.view(y * x, 1 << 26)[:, :f].reshape(1, y, x, f), want, bound + HALF_ULP["bf16"] * want.abs() * (1 + 2 ** -8))
+
+
 def test_nan_and_infinity_stay_in_their_group(eng):
     g = generator(13)
     data = random(g, 2, 5, 5, 32)

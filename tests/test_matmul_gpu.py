@@ -127,6 +127,26 @@ def test_nan_and_infinity_stay_in_their_rows(eng, size):
     op.close()
 
 
+@pytest.mark.parametrize("size,kernel", [
+    ((4090, 4093, 72), "tile<256x256>"), ((7160, 2040, 136), "tile<224x256>"), ((6130, 2046, 64), "tile<192x256>"), ((3100, 1537, 200), "tile<128x128>"),
+    ((1601, 1000, 104), "tile<64x128>"), ((1001, 1000, 264), "tile<64x64,k2>"), ((190, 2000, 520), "tile<32x64,k4>"), ((30, 1000, 1000), "split<16x16>"),
+    ((1001, 1000, 255), "tile<64x64,k2>"), ((600, 500, 63), "split<32x32>"), ((1601, 1400, 61), "split<64x64>"), ((3101, 1500, 263), "tile<64x128>"), ((3101, 1700, 263), "tile<128x128>")], ids=str)
+def test_every_kernel(eng, size, kernel):
+    m, n, k = size
+    dtype = "f16" if m % 2 else "bf16"
+    op = ops.Matmul(eng, ops.matmul_desc(m, n, k, dtype, bias=True, residual=True))
+    assert kernel in info(op) and op.info().launches == (2 if k % 8 and "tile" in kernel else 1)
+    op.close()
+    check(eng, m, n, k, dtype, act="gelu", residual=dtype)
+
+
+def test_pointers_that_are_not_aligned(eng):
+    # the description allows the tile kernels, the pointers do not
+    for size in ((300, 280, 64), (700, 600, 72)):
+        check(eng, *size, "f16", act="silu", offsets=(1, 0, 0, 0))
+        check(eng, *size, "f16", act="silu", offsets=(8, 3, 1, 0))
+
+
 def test_offsets_past_32_bits(eng):
     # rows 2^31 elements apart: the last of a starts 8 GiB in, that of the output 16 GiB
     m, n, k, pitch = 3, 33, 40, 1 << 31
