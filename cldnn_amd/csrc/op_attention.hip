@@ -7,6 +7,12 @@
 // the transposing LDS read gives, four keys of a value to a lane.
 // Values 16h + 4i + c of a block of 32 are put into row 8i + 4h + c of V^T, so a lane ends with 16 neighbouring values of its row.
 //
+// Measured (bf16, batch 4, 8 heads): 4096 x 4096 of 64 146 us (0.94 PFLOP/s), of 128 267 us (1.03); 3136 x 3136 of 64 105 us, where the
+// fullest CUs have two workgroups and the mean is 1.6.  The vector units are busy in two thirds of the time (32 exponentials at 8
+// clocks and 100 other instructions a tile and wave, 790 clocks), the matrix units in 43 % (512 clocks), at the 1.9 GHz that the power
+// limit leaves.  Scores of the next tile under the exponentials of this one were no faster (three waves to a SIMD instead of four).
+// One query over 50176 keys of 2 x 2 heads of 128: 24 us for lengths of 3/4 on average, 19 of it the keys at 4 TB/s.
+//
 // The waves of a workgroup share tiles of 64 keys, which direct loads bring into LDS one tile ahead.  Where rows are few the keys
 // are split over workgroups (of one wave then), and a second kernel joins their parts.
 #include "ops_common.h"

@@ -130,7 +130,8 @@ __device__ inline void matmul_meet()
 }
 
 // Few rows, or few tiles: 16 FT features x 16 PT rows to a workgroup, whose waves split K; both operands straight from memory into
-// the registers that the matrix instruction reads, U steps of 32 at a time; the partial sums meet in LDS.
+// the registers that the matrix instruction reads, U steps of 32 at a time; the partial sums meet in LDS.  Bound by the weights: 1 x
+// 25088 -> 4096 39 us, 5.3 TB/s, a large copy's rate; with 16 rows 55 us, their values being as many bytes again from the die's L2.
 template <typename T, int FT, int PT, int U, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void matmul_split_kernel(MatmulArgs a, const T* x, const T* w, void* out)
 {
@@ -209,6 +210,10 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_split_kernel(MatmulArgs a, 
 // buffers by direct loads, one step ahead of the one that is multiplied.  A row of 64 values is eight pieces of 16 bytes; piece c
 // of row r lies at place c ^ (r >> 1 & 7), so that the sixteen lanes that LDS serves at a time read all of its 64 banks.  Rows
 // behind the last are the last one again; pieces behind K are asked for behind the buffer's end, which gives zeros.
+// Measured (bf16): 8192 x 8192 x 8192 in 809 to 830 us on several cards, 1.33 to 1.36 PFLOP/s, the library's product 1.40; the matrix
+// units are busy in 72 % of the time, at the 1.5 GHz that the power limit leaves.  On the way there: 32x32x16 instructions 882 us,
+// both halves of the waves in step 926, tiles of a die in a row instead of a block 959.  25088 x 1024 -> 4096 with a gelu 232 us, its
+// product alone 203: seven rounds of 16 steps, 4 us of each the prologue and the stores, 4 the gelu, which nothing overlaps.
 // Row 16 t + r of a wave's 64 rows of weights is feature 16 (r / 4) + 4 t + r % 4 of its 64: the four results that the matrix
 // instruction leaves in a lane are neighbours, and so are those of the four blocks t: 16 features of one row of the result.
 template <typename T, int WM, int WN, int MB, int ST, int KG>

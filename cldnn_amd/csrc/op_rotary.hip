@@ -52,7 +52,8 @@ struct RotaryVector {
 
 // A thread turns W neighbouring pairs of a token in a group of its heads, queries' first, keys' behind them: one sine and cosine
 // for all of them, worked out while the first heads' values are on their way.  Their values are two runs of W, or where pairs are
-// interleaved one of 2 W.
+// interleaved one of 2 W.  Bound by memory: 25088 tokens with 16 + 4 heads of 128 (f16) 58 us, 4.4 TB/s where a large copy has 5.2
+// (a value at a time 80 us); in halves 63 us.  196 tokens with 16 + 16 heads of 64: 4.3 us, the launch.
 template <typename T, int W, bool INTERLEAVED>
 __global__ __launch_bounds__(ROTARY_THREADS) void rotary_kernel(RotaryArgs a, const RotaryPair* table, const void* positions, const T* q, const T* k, T* qo, T* ko)
 {
