@@ -450,7 +450,7 @@ MatmulPlan* matmul_plan(const cldnn_hip_engine_s& e, const cldnn_hip_matmul_desc
     plan->any = matmul_choose(d.m, d.n, false, cus);
     // The copy costs a launch and two trips of the operands, the kernels for any rows 5 times the tiles' time from there on (4000 x 255
     // -> 1000: 41 us without it, 10 with).
-    if (!whole && plan->any != MM_16 && (int64_t)d.m * d.n * d.k >= MATMUL_PACK && d.k < (1 << 20)) {
+    if (!whole && plan->any != MM_16 && d.k < (1 << 20) && (double)d.m * d.n * d.k >= MATMUL_PACK && ((int64_t)d.m + d.n) * ((d.k + 7) / 8) < (1ll << 38)) {
         plan->pieces = (d.k + 7) / 8;
         plan->kernel = matmul_choose(d.m, d.n, true, cus);
     }

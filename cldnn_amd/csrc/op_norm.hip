@@ -316,6 +316,7 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void norm_apply_kernel(NormArgs 
     });
 }
 
+constexpr size_t NORM_MOST_LDS = 64 << 10;
 static size_t norm_lds(const NormPlan& p) { return (p.a.rows * (p.a.span >> p.a.fold) + (p.whole ? p.a.span / p.a.cpg : 0)) * sizeof(float2); }
 
 NormPlan* norm_plan(const cldnn_hip_engine_s& e, const cldnn_hip_group_norm_desc& d, cldnn_hip_operator_info& info)
@@ -366,6 +367,8 @@ NormPlan* norm_plan(const cldnn_hip_engine_s& e, const cldnn_hip_group_norm_desc
         int threads = 256;
         while (threads < NORM_MOST_THREADS && (threads < vectors || (int64_t)a.P * vectors > 4ll * threads)) threads *= 2;
         shape(span, threads);
+        // (a feature to a group: its parts are the most there can be)
+        while (norm_lds(*plan) > NORM_MOST_LDS && threads > vectors && threads > 256) shape(span, threads /= 2);
         a.chunk = a.P;
     } else {
         shape(std::max(unit, std::min(NORM_MOST_SPAN, NORM_MOST_THREADS * V) / unit * unit), NORM_MOST_THREADS);

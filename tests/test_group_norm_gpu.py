@@ -68,6 +68,7 @@ def check(eng, x, groups, dtype, out, act="none", m=0.0, n=0.0, scale=None, shif
 SIZES = [  # b, y, x, f, groups
     (1, 1, 1, 8, 8), (1, 1, 1, 1, 1), (2, 1, 1, 64, 32), (1, 7, 7, 2048, 32), (3, 31, 45, 84, 12), (2, 56, 56, 64, 32), (1, 13, 9, 1369, 37),
     (5, 3, 2, 24, 1), (1, 112, 97, 16, 2), (2, 5, 3, 4160, 5), (1, 2, 3, 6144, 1), (1, 40, 40, 320, 32), (2, 17, 4, 26, 13), (33, 2, 2, 40, 4), (1, 4, 4, 3075, 3),
+    (1, 60, 60, 32, 32), (1, 130, 130, 32, 32), (2, 30, 20, 40, 40), (1, 70, 60, 16, 16),  # a feature to a group
 ]
 
 
