@@ -15,6 +15,8 @@ struct MatmulArgs {
     int32_t res_float, out_float;
     int32_t tiles, tiles_m, tiles_n;  // of the result
     int32_t band;                     // rows of tiles in a band
+    int32_t splits;                   // workgroups that split K for each tile: their sums go to part[split][m][n]
+    float* part;
 };
 
 constexpr int64_t MATMUL_PACK = 200ll << 20;  // products from which unaligned operands are copied
@@ -149,7 +151,8 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_split_kernel(MatmulArgs a, 
     for (int i = 0; i < FT; ++i) wr[i] = w + (int64_t)min(n0 + 16 * i + r, a.n - 1) * a.w_pitch + 8 * q;
     v4f acc[FT][PT] = {};
     const int whole = a.k / (32 * U);  // runs of U full steps, dealt to the waves in turn
-    for (int run = wave; run < whole; run += WAVES) {
+    const int worker = blockIdx.y * WAVES + wave, workers = a.splits * WAVES;
+    for (int run = worker; run < whole; run += workers) {
         const int k = run * 32 * U;
         v4i wf[U][FT], xf[U][PT];
 #pragma unroll
@@ -167,7 +170,9 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_split_kernel(MatmulArgs a, 
                 for (int j = 0; j < PT; ++j) acc[i][j] = mfma16(__builtin_bit_cast(V, wf[u][i]), __builtin_bit_cast(V, xf[u][j]), acc[i][j]);
     }
     // the steps behind the runs, one to a wave
-    for (int k = whole * 32 * U + 32 * ((wave - whole % WAVES + WAVES) % WAVES); k < a.k; k += 32 * WAVES) {
+    const int steps = a.k / 32 + (a.k % 32 != 0);
+    for (int step = whole * U + (worker - whole % workers + workers) % workers; step < steps; step += workers) {
+        const int k = step * 32;
         v4i wf[FT], xf[PT];
 #pragma unroll
         for (int i = 0; i < FT; ++i) wf[i] = matmul_load8(wr[i] - 8 * q, k + 8 * q, a.k);
@@ -195,6 +200,10 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_split_kernel(MatmulArgs a, 
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] += sums[s][at + i];
         const int row = at / (16 * FT), n = n0 + at - row * 16 * FT;
+        if (a.splits > 1) {
+            if (m0 + row < a.m && n < a.n) matmul_write(a.part + ((int64_t)blockIdx.y * a.m + m0 + row) * a.n + n, a.n - n, v);
+            continue;
+        }
         if (a.bias && n < a.n) {
             float b[N];
             matmul_read(a.bias + n, a.n - n, b);
@@ -204,6 +213,31 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_split_kernel(MatmulArgs a, 
         act_apply(v, a.act);
         matmul_write_row<T>(a, v, m0 + row, n, out);
     }
+}
+
+// The sums of the workgroups that split K, joined in their order: four features of a row to a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void matmul_join_kernel(MatmulArgs a, void* out)
+{
+    const int across = (a.n + 3) / 4, i = blockIdx.x * 256 + threadIdx.x, m = i / across, n = (i - m * across) * 4;
+    if (m >= a.m) return;
+    float v[4];
+    matmul_read(a.part + (int64_t)m * a.n + n, a.n - n, v);
+#pragma unroll 4
+    for (int s = 1; s < a.splits; ++s) {
+        float x[4];
+        matmul_read(a.part + ((int64_t)s * a.m + m) * a.n + n, a.n - n, x);
+#pragma unroll
+        for (int l = 0; l < 4; ++l) v[l] += x[l];
+    }
+    if (a.bias) {
+        float b[4];
+        matmul_read(a.bias + n, a.n - n, b);
+#pragma unroll
+        for (int l = 0; l < 4; ++l) v[l] += b[l];
+    }
+    act_apply(v, a.act);
+    matmul_write_row<T>(a, v, m, n, out);
 }
 
 // BM x BN of the result to a workgroup of WM x WN waves, 16 MB rows x 64 features to a wave.  Both operands come 64 deep into two LDS
@@ -456,11 +490,16 @@ MatmulPlan* matmul_plan(const cldnn_hip_engine_s& e, const cldnn_hip_matmul_desc
     }
     const MatmulKernel& kernel = matmul_kernels[plan->kernel];
     matmul_tiles(a, kernel);
-    info.launches = plan->pieces ? 2 : 1, info.block = 64 * kernel.waves, info.grid = a.tiles;
-    info.workspace_bytes = ((int64_t)d.m + d.n) * plan->pieces * 16;
+    // The smallest tiles that leave half of the chip idle over a long K: several workgroups to a tile, for the price of a second launch.
+    // Without it and with it: 16 x 1000 x 25088 44.9 and 20.3 us, 1 x 500 x 25088 29.0 and 10.8, 8 x 1000 x 16384 24.9 and 12.4,
+    // 4 x 2000 x 8000 12.5 and 11.6; 1 x 1000 x 4096 6.6 and 9.3, so from 8000 on.
+    a.splits = 1;
+    if (plan->kernel == MM_16 && a.tiles * 2 <= cus && d.k >= 8000) a.splits = std::min(cus / a.tiles, d.k / 2048);
+    info.launches = plan->pieces || a.splits > 1 ? 2 : 1, info.block = 64 * kernel.waves, info.grid = a.tiles * a.splits;
+    info.workspace_bytes = ((int64_t)d.m + d.n) * plan->pieces * 16 + (a.splits > 1 ? (int64_t)a.splits * d.m * d.n * 4 : 0);
     info.ops = 2ll * d.m * d.n * d.k;
     info.bytes = 2 * ((int64_t)d.m * d.k + (int64_t)d.n * d.k) + (d.has_bias ? 4ll * d.n : 0) + (int64_t)d.m * d.n * (out_size + res_size);
-    snprintf(info.kernel_name, sizeof info.kernel_name, "%s", kernel.name);
+    snprintf(info.kernel_name, sizeof info.kernel_name, "%s%s", kernel.name, a.splits > 1 ? " + matmul_join" : "");
     return plan.release();
 }
 
@@ -474,6 +513,7 @@ void matmul_launch(hipStream_t s, const MatmulPlan& p, void* workspace, const vo
     with_half(p.dt, [&](auto t) {
         typedef decltype(t) T;
         const void *xa = x, *wa = w;
+        a.part = (float*)workspace;
         if (p.pieces) {
             const int64_t blocks = (((int64_t)a.m + a.n) * p.pieces + 255) / 256;
             hipLaunchKernelGGL((matmul_pack_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a, (const T*)x, (const T*)w, (v4i*)workspace, p.pieces);
@@ -483,7 +523,7 @@ void matmul_launch(hipStream_t s, const MatmulPlan& p, void* workspace, const vo
         const int row = (((uintptr_t)xa | (uintptr_t)wa) & 15) == 0 ? p.kernel : p.any;
         const MatmulKernel& kernel = matmul_kernels[row];
         matmul_tiles(a, kernel);
-        const auto launch = [&](auto f) { hipLaunchKernelGGL(f, dim3(a.tiles), dim3(64 * kernel.waves), 0, s, a, (const T*)xa, (const T*)wa, out); };
+        const auto launch = [&](auto f) { hipLaunchKernelGGL(f, dim3(a.tiles, a.splits), dim3(64 * kernel.waves), 0, s, a, (const T*)xa, (const T*)wa, out); };
         switch (row) {
         case MM_256: launch(matmul_tile_kernel<T, 2, 4, 8, 2, 1>); break;
         case MM_224: launch(matmul_tile_kernel<T, 2, 4, 7, 2, 1>); break;
@@ -496,6 +536,8 @@ void matmul_launch(hipStream_t s, const MatmulPlan& p, void* workspace, const vo
         case MM_ANY_32: launch(matmul_split_kernel<T, 2, 2, 4, 8>); break;
         default: launch(matmul_split_kernel<T, 1, 1, 16, 8>);
         }
+        if (a.splits > 1)
+            hipLaunchKernelGGL((matmul_join_kernel<T>), dim3((unsigned)(((int64_t)a.m * ((a.n + 3) / 4) + 255) / 256)), dim3(256), 0, s, a, out);
     });
     CHIP_CHECK(hipGetLastError());
 }

@@ -130,14 +130,18 @@ def test_nan_and_infinity_stay_in_their_rows(eng, size):
 @pytest.mark.parametrize("size,kernel", [
     ((4090, 4093, 72), "tile<256x256>"), ((7160, 2040, 136), "tile<224x256>"), ((6130, 2046, 64), "tile<192x256>"), ((3100, 1537, 200), "tile<128x128>"),
     ((1601, 1000, 104), "tile<64x128>"), ((1001, 1000, 264), "tile<64x64,k2>"), ((190, 2000, 520), "tile<32x64,k4>"), ((30, 1000, 1000), "split<16x16>"),
+    ((7, 250, 9000), "split<16x16> + matmul_join"), ((1, 31, 16383), "split<16x16> + matmul_join"), ((20, 65, 8200), "split<16x16> + matmul_join"),
     ((1001, 1000, 255), "tile<64x64,k2>"), ((600, 500, 63), "split<32x32>"), ((1601, 1400, 61), "split<64x64>"), ((3101, 1500, 263), "tile<64x128>"), ((3101, 1700, 263), "tile<128x128>")], ids=str)
 def test_every_kernel(eng, size, kernel):
     m, n, k = size
     dtype = "f16" if m % 2 else "bf16"
     op = ops.Matmul(eng, ops.matmul_desc(m, n, k, dtype, bias=True, residual=True))
-    assert kernel in info(op) and op.info().launches == (2 if k % 8 and "tile" in kernel else 1)
+    assert kernel in info(op) and op.info().launches == (2 if k % 8 and "tile" in kernel or "join" in kernel else 1)
     op.close()
     check(eng, m, n, k, dtype, act="gelu", residual=dtype)
+    if "join" in kernel:
+        check(eng, m, n, k, dtype, out="f32", act="relu", residual="f32", act2="silu", in_place=True)
+        check(eng, m, n, k, dtype, bias=False, spare=(1, 0, 3, 0), offsets=(1, 3, 0, 0))
 
 
 def test_pointers_that_are_not_aligned(eng):
