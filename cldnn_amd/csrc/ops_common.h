@@ -44,10 +44,12 @@ __device__ inline uint32_t lds_address(const v4i* p) { return (uint32_t)(uintptr
 // Lane t's 16 bytes at `offset` + `step` go to LDS at place t from `to` on.  Written out because the compiler, where it issues this
 // load itself, waits for all loads under way in front of one of three LDS reads of a loop (1498 against 1090 us for 8192 x 8192 x
 // 8192).  It has no result in registers; a wait for vmcnt, written out as well, is what it needs before anybody reads.
-// M0, which it sets, has no other user in these kernels: this device's LDS instructions do not read it, and no register is indexed.
+// The load takes its place from M0, and a scalar write of M0 needs a wait state in front of it, which the compiler leaves for its own
+// loads and does not look for in here.
+// M0 has no other user in these kernels: this device's LDS instructions do not read it, and no register is indexed.
 __device__ inline void load_lds(v4i from, uint32_t to, int offset, int step)
 {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(offset), "s"(from), "s"(step) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(offset), "s"(from), "s"(step) : "memory");
 }
 
 // ----------------------------------------------------------------------------- activations
