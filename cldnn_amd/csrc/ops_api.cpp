@@ -66,6 +66,16 @@ void check(cldnn_hip_operator op, OperatorKind kind)
     CHIP_REQUIRE(op->kind == kind, CLDNN_HIP_INVALID_ARG, "an operator of another kind");
 }
 
+// launch(): the call's kernels, in one piece where they hand each other the object's scratch memory
+template <typename F>
+void enqueue(cldnn_hip_operator op, F&& launch)
+{
+    op->engine->make_current();
+    std::unique_lock<std::mutex> alone(op->engine->together, std::defer_lock);
+    if (op->info.launches > 1) alone.lock();
+    launch(op->engine->launch_stream());
+}
+
 }  // namespace
 
 extern "C" {
@@ -121,8 +131,7 @@ cldnn_hip_status cldnn_hip_group_norm_enqueue(cldnn_hip_operator op, const void*
     return guarded([&] {
         check(op, OP_GROUP_NORM);
         CHIP_REQUIRE(input_dev && output_dev, CLDNN_HIP_INVALID_ARG, "null device pointer");
-        op->engine->make_current();
-        norm_launch(op->engine->launch_stream(), *op->norm, op->workspace, input_dev, scale_dev, shift_dev, output_dev);
+        enqueue(op, [&](hipStream_t s) { norm_launch(s, *op->norm, op->workspace, input_dev, scale_dev, shift_dev, output_dev); });
     });
 }
 
@@ -137,8 +146,7 @@ cldnn_hip_status cldnn_hip_matmul_enqueue(cldnn_hip_operator op, const void* a_d
     return guarded([&] {
         check(op, OP_MATMUL);
         CHIP_REQUIRE(a_dev && weights_dev && output_dev, CLDNN_HIP_INVALID_ARG, "null device pointer");
-        op->engine->make_current();
-        matmul_launch(op->engine->launch_stream(), *op->matmul, op->workspace, a_dev, weights_dev, bias_dev, residual_dev, output_dev);
+        enqueue(op, [&](hipStream_t s) { matmul_launch(s, *op->matmul, op->workspace, a_dev, weights_dev, bias_dev, residual_dev, output_dev); });
     });
 }
 
@@ -153,8 +161,7 @@ cldnn_hip_status cldnn_hip_rotary_enqueue(cldnn_hip_operator op, const void* q_d
     return guarded([&] {
         check(op, OP_ROTARY);
         CHIP_REQUIRE(q_dev && q_out_dev && positions_dev, CLDNN_HIP_INVALID_ARG, "null device pointer");
-        op->engine->make_current();
-        rotary_launch(op->engine->launch_stream(), *op->rotary, op->workspace, q_dev, k_dev, positions_dev, q_out_dev, k_out_dev);
+        enqueue(op, [&](hipStream_t s) { rotary_launch(s, *op->rotary, op->workspace, q_dev, k_dev, positions_dev, q_out_dev, k_out_dev); });
     });
 }
 
@@ -169,8 +176,7 @@ cldnn_hip_status cldnn_hip_attention_enqueue(cldnn_hip_operator op, const void* 
     return guarded([&] {
         check(op, OP_ATTENTION);
         CHIP_REQUIRE(q_dev && k_dev && v_dev && output_dev, CLDNN_HIP_INVALID_ARG, "null device pointer");
-        op->engine->make_current();
-        attention_launch(op->engine->launch_stream(), *op->attention, op->workspace, q_dev, k_dev, v_dev, key_lengths_dev, bias_dev, output_dev);
+        enqueue(op, [&](hipStream_t s) { attention_launch(s, *op->attention, op->workspace, q_dev, k_dev, v_dev, key_lengths_dev, bias_dev, output_dev); });
     });
 }
 

@@ -357,6 +357,7 @@ cldnn_hip_status cldnn_hip_recording_enqueue(cldnn_hip_recording r)
         CHIP_REQUIRE(capture == hipStreamCaptureStatusNone && r->engine->launch_stream() == r->engine->stream, CLDNN_HIP_ERROR,
                      "a recording is not enqueued into a capture");
         r->engine->make_current();
+        std::lock_guard<std::mutex> g(r->engine->together);
         CHIP_CHECK(hipGraphLaunch(r->exec, r->engine->stream));
     });
 }

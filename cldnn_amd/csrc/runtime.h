@@ -27,6 +27,10 @@ struct cldnn_hip_engine_s {
     uint64_t marks = 0;
     uint64_t* reached = nullptr;
 
+    // Held over the launches of a call whose kernels hand each other an object's scratch memory, and over a recording's, which may
+    // hold such a call: no other thread's lie between them on the stream.
+    std::mutex together;
+
     hipEvent_t take_event();
     void give_event(hipEvent_t ev);
     uint64_t mark();

@@ -1,0 +1,119 @@
+"""What the float operators' library does on the host, with a runtime that only writes launches down (tests/cpp/host_runtime.cpp):
+the order of launches from several threads.  No GPU: each test is a process of its own."""
+import ctypes as C
+import os
+import subprocess
+import sys
+import threading
+
+import pytest
+
+from cldnn_amd import hip, ops
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+ROOT = os.path.dirname(HERE)
+ROCM = "/opt/rocm/include"
+pytestmark = pytest.mark.skipif(not os.path.exists(os.path.join(ROCM, "hip")), reason="needs the runtime's headers")
+
+
+@pytest.fixture(scope="module")
+def runtime(tmp_path_factory):
+    path = str(tmp_path_factory.mktemp("host") / "runtime.so")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-I", ROCM, os.path.join(HERE, "cpp", "host_runtime.cpp"), "-o", path],
+                   check=True)
+    return path
+
+
+@pytest.fixture
+def on_host(runtime):
+    """runs a function of this module in a process whose runtime is the host's"""
+    def run(function, *args):
+        code = "import sys; sys.path[:0] = %r; import test_operators_host as t; t.%s(*%r)" % ([ROOT, HERE], function.__name__, args)
+        env = dict(os.environ, LD_PRELOAD=":".join(x for x in (runtime, os.environ.get("LD_PRELOAD")) if x))
+        p = subprocess.run([sys.executable, "-c", code], env=env, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=120)
+        assert p.returncode == 0, p.stdout
+    return run
+
+
+# ---------------------------------------------------------------------------------------------------- in the other process
+AT = 1 << 20  # stands for device memory: nothing reads it
+
+
+def host():
+    return C.CDLL(None)
+
+
+def launches():
+    """[(thread, kernel, workgroups, threads of one, bytes of dynamic LDS)] since the start"""
+    h, name, shape, found = host(), C.create_string_buffer(1024), (C.c_uint * 3)(), []
+    h.host_launch.restype = C.c_size_t
+    for i in range(h.host_launches()):
+        thread = h.host_launch(i, name, len(name), shape)
+        found.append((thread, name.value.decode(), *shape))
+    return found
+
+
+def calls_of_two_kernels(e):
+    """name -> (operator, a call of it)"""
+    made = {
+        "norm": (ops.GroupNorm(e, ops.group_norm_desc(ops.map_tensor("f16", 1, 90, 80, 64), 8)), (AT, AT)),
+        "packed": (ops.Matmul(e, ops.matmul_desc(1001, 1000, 255, "f16")), (AT, AT, AT)),
+        "joined": (ops.Matmul(e, ops.matmul_desc(7, 250, 9000, "f16")), (AT, AT, AT)),
+        "attention": (ops.Attention(e, ops.attention_desc(1, 1, 5000, 8, 2, 64, "f16")), (AT, AT, AT, AT)),
+    }
+    for op, _ in made.values():
+        assert op.info().launches == 2 and op.info().workspace_bytes
+    return {k: (op, lambda op=op, args=args: op.enqueue(*args)) for k, (op, args) in made.items()}
+
+
+def two_threads(name):
+    e = hip.Engine()
+    op, call = calls_of_two_kernels(e)[name]
+    call()
+    pair = [l[1] for l in launches()]
+    assert len(pair) == 2 and pair[0] != pair[1]
+    host().host_pause(300)
+
+    def work():
+        for _ in range(30):
+            call()
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    found = launches()[2:]
+    assert len(found) == 120
+    # the second kernel of a call reads what its first one left in the object's memory
+    for first, second in zip(found[::2], found[1::2]):
+        assert [first[1], second[1]] == pair and first[0] == second[0], "a launch of the other thread between the kernels of a call"
+
+
+@pytest.mark.parametrize("name", ["norm", "packed", "joined", "attention"])
+def test_threads_that_enqueue_one_operator(on_host, name):
+    on_host(two_threads, name)
+
+
+def a_thread_and_a_recording():
+    e = hip.Engine()
+    op, call = calls_of_two_kernels(e)["attention"]
+    L, rec = hip.lib(), C.c_void_p()
+    hip.check(L.cldnn_hip_engine_record_begin(e.h))
+    call()
+    hip.check(L.cldnn_hip_engine_record_end(e.h, C.byref(rec)))
+    host().host_pause(300)
+    thread = threading.Thread(target=lambda: [hip.check(L.cldnn_hip_recording_enqueue(rec)) for _ in range(40)])
+    thread.start()
+    for _ in range(40):
+        call()
+    thread.join()
+    found = [l[1] for l in launches()]
+    assert len(found) == 120 and found.count("graph") == 40
+    for i, name in enumerate(found):
+        if "attention_join" in name:
+            assert found[i - 1] != "graph", "a recording between the kernels of a call"
+
+
+def test_a_thread_enqueues_and_another_a_recording(on_host):
+    on_host(a_thread_and_a_recording)
