@@ -73,6 +73,11 @@ void enqueue(cldnn_hip_operator op, F&& launch)
     op->engine->make_current();
     std::unique_lock<std::mutex> alone(op->engine->together, std::defer_lock);
     if (op->info.launches > 1) alone.lock();
+    // a recording's kernels go on using the object's memory: it holds the object
+    if (op->workspace && op->engine->launch_stream() != op->engine->stream) {
+        (void)cldnn_hip_operator_retain(op);
+        op->engine->hold([op] { (void)cldnn_hip_operator_release(op); });
+    }
     launch(op->engine->launch_stream());
 }
 

@@ -103,14 +103,20 @@ void cldnn_hip_buffer_s::upload()
     CHIP_CHECK(hipMemcpyAsync(dev, shadow, bytes, hipMemcpyHostToDevice, engine->stream));
 }
 
-// one recording to a thread: its engine, and the stream that collects the launches
+// one recording to a thread: its engine, the stream that collects the launches, and how to give back what they need
 struct thread_recording {
     cldnn_hip_engine engine = nullptr;
     hipStream_t stream = nullptr;
+    std::vector<std::function<void()>> held;
 };
 static thread_local thread_recording g_recording;
 
 hipStream_t cldnn_hip_engine_s::launch_stream() const { return g_recording.engine == this ? g_recording.stream : stream; }
+
+void cldnn_hip_engine_s::hold(std::function<void()> release) const
+{
+    if (g_recording.engine == this) g_recording.held.push_back(std::move(release));
+}
 
 void cldnn_hip_engine_s::make_current() const { CHIP_CHECK(hipSetDevice(device)); }
 
@@ -317,7 +323,7 @@ cldnn_hip_status cldnn_hip_engine_record_begin(cldnn_hip_engine e)
             (void)hipStreamDestroy(s);
             CHIP_CHECK(r);
         }
-        g_recording = {e, s};
+        g_recording.engine = e, g_recording.stream = s;
         e->refs.fetch_add(1);
     });
 }
@@ -328,6 +334,7 @@ cldnn_hip_status cldnn_hip_engine_record_end(cldnn_hip_engine e, cldnn_hip_recor
     return guarded([&] {
         CHIP_REQUIRE(e && g_recording.engine == e, CLDNN_HIP_INVALID_ARG, "this thread is not recording on that engine");
         const hipStream_t s = g_recording.stream;
+        std::vector<std::function<void()>> held = std::move(g_recording.held);
         g_recording = {};
         hipGraph_t graph = nullptr;
         hipGraphExec_t exec = nullptr;
@@ -338,12 +345,13 @@ cldnn_hip_status cldnn_hip_engine_record_end(cldnn_hip_engine e, cldnn_hip_recor
         (void)hipStreamDestroy(s);
         if (r != hipSuccess || !out) {
             if (exec) (void)hipGraphExecDestroy(exec);
+            for (const auto& release : held) release();
             cldnn_hip_engine_release(e);
             CHIP_CHECK(r);
             return;
         }
         auto* rec = new cldnn_hip_recording_s();
-        rec->engine = e, rec->exec = exec;
+        rec->engine = e, rec->exec = exec, rec->held = std::move(held);
         *out = rec;
     });
 }
@@ -370,6 +378,7 @@ cldnn_hip_status cldnn_hip_recording_release(cldnn_hip_recording r)
         (void)hipSetDevice(e->device);
         (void)hipStreamSynchronize(e->stream);
         (void)hipGraphExecDestroy(r->exec);
+        for (const auto& release : r->held) release();
         delete r;
         cldnn_hip_engine_release(e);
     });

@@ -2,6 +2,7 @@
 #pragma once
 #include <atomic>
 #include <condition_variable>
+#include <functional>
 #include <mutex>
 #include <utility>
 #include <vector>
@@ -39,12 +40,16 @@ struct cldnn_hip_engine_s {
     void make_current() const;
     // where a launch of this thread goes: the stream, or what the thread is recording (cldnn_hip_engine_record_begin)
     hipStream_t launch_stream() const;
+    // what a call that goes into this thread's recording needs for as long as that lasts: `release` is called behind it.  Nothing to do
+    // where the thread does not record.
+    void hold(std::function<void()> release) const;
 };
 
 // The launches of a recording as an instantiated graph.
 struct cldnn_hip_recording_s {
     cldnn_hip_engine engine = nullptr;
     hipGraphExec_t exec = nullptr;
+    std::vector<std::function<void()>> held;
 };
 
 struct cldnn_hip_buffer_s {

@@ -8,8 +8,10 @@
  * with cldnn_hip_engine_record_begin or captured).  Calls of one object share its scratch and may not overlap.  Those made
  * through the library never do, whichever threads make them: the kernels of a call, and those of a recording, follow each
  * other on the engine's stream.  A graph that the application captured itself has to run on that stream too, and not be
- * launched while another thread enqueues the object.  Every entry point returns a cldnn_hip_status; the message of the last failure is
- * cldnn_hip_last_error().  Exported by libcldnn_hip_ops.so, which needs libcldnn_hip.so.
+ * launched while another thread enqueues the object.  A recording holds the operators whose memory its kernels use until
+ * it is released; an operator in a graph that the application captured has to outlive the graph.  Every entry point
+ * returns a cldnn_hip_status; the message of the last failure is cldnn_hip_last_error().  Exported by
+ * libcldnn_hip_ops.so, which needs libcldnn_hip.so.
  *
  * Floating types: sums, statistics and softmax are held in 32 bits whatever the type of the data; results are rounded
  * once, to nearest even, unless stated otherwise.  Pointers need the alignment of one element; strides count elements.

@@ -117,3 +117,37 @@ def a_thread_and_a_recording():
 
 def test_a_thread_enqueues_and_another_a_recording(on_host):
     on_host(a_thread_and_a_recording)
+
+
+def memory():
+    host().host_memory.restype = C.c_size_t
+    return host().host_memory()
+
+
+def a_recording_outlives_its_operators(kept):
+    e = hip.Engine()
+    L, rec, before = hip.lib(), C.c_void_p(), memory()
+    calls = calls_of_two_kernels(e)
+    scratch = sum(op.info().workspace_bytes for op, _ in calls.values())
+    assert memory() - before == scratch
+    hip.check(L.cldnn_hip_engine_record_begin(e.h))
+    for _, call in calls.values():
+        call()
+        call()
+    hip.check(L.cldnn_hip_engine_record_end(e.h, C.byref(rec) if kept else None))
+    for op, _ in calls.values():
+        op.close()
+    assert memory() - before == (scratch if kept else 0), "the scratch memory of a recording's kernels"
+    if kept:
+        e.close()
+        hip.check(L.cldnn_hip_recording_enqueue(rec))
+        hip.check(L.cldnn_hip_recording_release(rec))
+        assert memory() == 0  # the engine's, too
+    else:
+        e.close()
+        assert memory() == 0
+
+
+@pytest.mark.parametrize("kept", [True, False])
+def test_a_recording_holds_the_operators_in_it(on_host, kept):
+    on_host(a_recording_outlives_its_operators, kept)
