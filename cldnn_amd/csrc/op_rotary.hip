@@ -2,7 +2,9 @@
 //
 // angle = position * frequency is held in turns: with frequency / (2 pi) as the sum of two floats hi + lo (worked out in 64 bits
 // when the object is made), position * hi is split exactly into its rounded product and the rest, the whole turns are dropped
-// from the product, and what is left is below one turn and good to about 2^-24 of a turn whatever the position.
+// from the product, and what is left is below one turn and good to about 2^-24 of a turn as long as position * frequency is below
+// 2^24: for every position that a float has exactly, where the base is 1 or more.  (Beyond, the rest is whole turns itself, and the
+// frequency's own 48 bits are too few: position 2^24, base 1e-4: 2^-13 of a turn.)
 #include <cmath>
 
 #include "ops_common.h"

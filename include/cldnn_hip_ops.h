@@ -97,8 +97,8 @@ cldnn_hip_status cldnn_hip_matmul_enqueue(cldnn_hip_operator op, const void* a_d
  * Each head's first 2 * (pairs of all axes) values are pairs that turn with the token's position along one axis:
  *   angle = position[token][axis] * base^-(exponent),  y0 = x0 cos - x1 sin,  y1 = x1 cos + x0 sin;
  * the values behind them are copied.  Axis 0 has the first pairs, and so on.  The exponent of pair i, the j-th of its
- * axis' J, is j / J, or i / (pairs of all axes) with shared_frequencies.  Angles are exact to 32 bits for positions
- * up to 2^24 in magnitude. */
+ * axis' J, is j / J, or i / (pairs of all axes) with shared_frequencies.  Angles are good to 2^-24 of a turn for
+ * positions up to 2^24 in magnitude; with a base below 1, whose frequencies go up to 1 / base, up to 2^24 * base. */
 #define CLDNN_HIP_ROTARY_MAX_AXES 4
 enum {
     CLDNN_HIP_ROTARY_INTERLEAVED = 0,     /* pair i: values 2i, 2i + 1 */

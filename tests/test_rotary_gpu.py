@@ -108,6 +108,16 @@ def test_large_and_fractional_positions(eng):
     check(eng, 64, 2, 2, 64, (16, 16), "f32", positions=torch.zeros(64, 2, dtype=torch.int32))
 
 
+@pytest.mark.parametrize("base", [0.5, 2.0 ** -7, 2.0 ** -13])
+def test_bases_below_one(eng, base):
+    # frequencies up to 1 / base, positions up to 2^24 * base
+    most = int(2 ** 24 * base)
+    positions = torch.randint(-most, most + 1, (64, 2), generator=generator(7), dtype=torch.int32)
+    positions[0] = torch.tensor([most, -most])
+    check(eng, 64, 2, 2, 64, (16, 16), "f32", positions=positions, base=base)
+    check(eng, 64, 2, 2, 64, (12, 20), "f32", positions=positions.float() * 0.75, base=base, shared=True)
+
+
 def test_gradient(eng):
     """The transpose of a rotation is the rotation back: against automatic differentiation of the formula, and against differences
     (the operator is linear: they are exact but for its roundings)."""
