@@ -168,6 +168,37 @@ def test_offsets_past_32_bits(eng):
     op.close()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("size,kernel", [
+    ((1, 1000, 2048), "split<16x16>"), ((1, 33, 4100), "split<16x16>"), ((3, 40, 1031), "split<16x16>"), ((16, 4096, 25088), "split<16x16>"), ((40, 40, 16384), "join"), ((1, 31, 16383), "join"),
+    ((20, 65, 8200), "join"), ((7, 250, 9001), "join"), ((9, 100, 20480), "join"), ((600, 500, 63), "split<32x32>"), ((190, 2000, 2056), "tile<32x64,k4>"), ((1001, 1000, 1992), "tile<64x64,k2>"),
+    ((1001, 1000, 2055), "matmul_tile<64x64,k2>"), ((1601, 1000, 1096), "tile<64x128>"), ((3100, 1537, 1064), "tile<128x128>"), ((4090, 4093, 1032), "tile<256x256>"), ((6130, 2046, 1000), "tile<192x256>"),
+    ((7160, 2040, 1160), "tile<224x256>")], ids=str)
+def test_sums_of_whole_numbers_are_exact(eng, size, kernel, dtype):
+    """Whose partial sums all fit 32 bits and do not fit 16: no value of K may be lost, and no sum held in fewer bits, at any length.
+    No value is zero, so every k counts."""
+    m, n, k = size
+    g = generator(sum(size))
+    a = torch.randint(1, 4, (m, k), generator=g).to(TYPES[dtype])
+    w = torch.tensor([-1, 1, 2, 3])[torch.randint(0, 4, (n, k), generator=g)].to(TYPES[dtype])
+    want = a.double() @ w.double().T  # at most 9 k, exact in any order
+    assert 9 * k < 1 << 24
+    op = ops.Matmul(eng, ops.matmul_desc(m, n, k, dtype, out_dtype="f32"))
+    assert kernel in info(op)
+    out = torch.full((m, n), math.nan, device="cuda")
+    run(eng, op, a.cuda(), w.cuda(), out)
+    assert torch.equal(out.cpu().double(), want)
+    op.close()
+    if k % 8 == 0:  # the kernel for any rows
+        op = ops.Matmul(eng, ops.matmul_desc(m, n, k, dtype, out_dtype="f32", a_stride=k + 1))
+        far = torch.full((m, k + 1), math.nan, dtype=a.dtype)
+        far[:, :k] = a
+        out.fill_(math.nan)
+        run(eng, op, far.cuda(), w.cuda(), out)
+        assert torch.equal(out.cpu().double(), want)
+        op.close()
+
+
 def test_refusals(eng):
     def status(*args, **kw):
         return refused(eng, ops.Matmul, ops.matmul_desc(*args, **kw))
