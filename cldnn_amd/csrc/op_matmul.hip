@@ -20,6 +20,7 @@ struct MatmulArgs {
 };
 
 constexpr int64_t MATMUL_PACK = 200ll << 20;  // products from which unaligned operands are copied
+constexpr int MATMUL_PACK_THREADS = 256;
 
 struct MatmulPlan {
     MatmulArgs a;
@@ -400,9 +401,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG, KG > 2 ? KG : 2) void matmul_til
 
 // Operands whose rows are no whole 16-byte pieces, copied into rows that are, zeros behind K: row i of a, then row j of weights.
 template <typename T>
-__global__ __launch_bounds__(256) void matmul_pack_kernel(MatmulArgs a, const T* x, const T* w, v4i* to, int pieces)
+__global__ __launch_bounds__(MATMUL_PACK_THREADS) void matmul_pack_kernel(MatmulArgs a, const T* x, const T* w, v4i* to, int pieces)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / pieces;
+    const int64_t i = (int64_t)blockIdx.x * MATMUL_PACK_THREADS + threadIdx.x, row = i / pieces;
     const int k = (int)(i - row * pieces) * 8;
     if (row >= a.m + a.n) return;
     to[i] = matmul_load8(row < a.m ? x + row * a.a_pitch : w + (row - a.m) * a.w_pitch, k, a.k);
@@ -411,13 +412,17 @@ __global__ __launch_bounds__(256) void matmul_pack_kernel(MatmulArgs a, const T*
 struct MatmulKernel {
     const char* name;
     int rows, features, waves;
+    int lds;  // bytes: the stages of both operands, or the waves' sums
 };
 enum { MM_256, MM_224, MM_192, MM_128, MM_64x128, MM_64, MM_32, MM_ANY_64, MM_ANY_32, MM_16 };
 static const MatmulKernel matmul_kernels[] = {
-    {"matmul_tile<256x256>", 256, 256, 8}, {"matmul_tile<224x256>", 224, 256, 8}, {"matmul_tile<192x256>", 192, 256, 8},
-    {"matmul_tile<128x128>", 128, 128, 4}, {"matmul_tile<64x128>", 64, 128, 4}, {"matmul_tile<64x64,k2>", 64, 64, 8}, {"matmul_tile<32x64,k4>", 32, 64, 8},
-    {"matmul_split<64x64>", 64, 64, 4}, {"matmul_split<32x32>", 32, 32, 8}, {"matmul_split<16x16>", 16, 16, 8},
+    {"matmul_tile<256x256>", 256, 256, 8, 128 << 10}, {"matmul_tile<224x256>", 224, 256, 8, 120 << 10}, {"matmul_tile<192x256>", 192, 256, 8, 112 << 10},
+    {"matmul_tile<128x128>", 128, 128, 4, 64 << 10}, {"matmul_tile<64x128>", 64, 128, 4, 72 << 10},
+    {"matmul_tile<64x64,k2>", 64, 64, 8, 128 << 10}, {"matmul_tile<32x64,k4>", 32, 64, 8, 144 << 10},
+    {"matmul_split<64x64>", 64, 64, 4, 64 << 10}, {"matmul_split<32x32>", 32, 32, 8, 32 << 10}, {"matmul_split<16x16>", 16, 16, 8, 8 << 10},
 };
+
+static int64_t matmul_pack_blocks(const MatmulPlan& p) { return (((int64_t)p.a.m + p.a.n) * p.pieces + MATMUL_PACK_THREADS - 1) / MATMUL_PACK_THREADS; }
 
 static int64_t matmul_count(int m, int n, const MatmulKernel& k) { return (int64_t)((m + k.rows - 1) / k.rows) * ((n + k.features - 1) / k.features); }
 
@@ -495,11 +500,12 @@ MatmulPlan* matmul_plan(const cldnn_hip_engine_s& e, const cldnn_hip_matmul_desc
     // 4 x 2000 x 8000 12.5 and 11.6; 1 x 1000 x 4096 6.6 and 9.3, so from 8000 on.
     a.splits = 1;
     if (plan->kernel == MM_16 && a.tiles * 2 <= cus && d.k >= 8000) a.splits = std::min(cus / a.tiles, d.k / 2048);
-    info.launches = plan->pieces || a.splits > 1 ? 2 : 1, info.block = 64 * kernel.waves, info.grid = a.tiles * a.splits;
+    info.launches = plan->pieces || a.splits > 1 ? 2 : 1, info.block = 64 * kernel.waves, info.grid = a.tiles * a.splits, info.lds_bytes = kernel.lds;
+    if (plan->pieces) info.block = MATMUL_PACK_THREADS, info.grid = (int32_t)matmul_pack_blocks(*plan);
     info.workspace_bytes = ((int64_t)d.m + d.n) * plan->pieces * 16 + (a.splits > 1 ? (int64_t)a.splits * d.m * d.n * 4 : 0);
     info.ops = 2ll * d.m * d.n * d.k;
     info.bytes = 2 * ((int64_t)d.m * d.k + (int64_t)d.n * d.k) + (d.has_bias ? 4ll * d.n : 0) + (int64_t)d.m * d.n * (out_size + res_size);
-    snprintf(info.kernel_name, sizeof info.kernel_name, "%s%s", kernel.name, a.splits > 1 ? " + matmul_join" : "");
+    snprintf(info.kernel_name, sizeof info.kernel_name, "%s%s%s", plan->pieces ? "matmul_pack + " : "", kernel.name, a.splits > 1 ? " + matmul_join" : "");
     return plan.release();
 }
 
@@ -515,8 +521,7 @@ void matmul_launch(hipStream_t s, const MatmulPlan& p, void* workspace, const vo
         const void *xa = x, *wa = w;
         a.part = (float*)workspace;
         if (p.pieces) {
-            const int64_t blocks = (((int64_t)a.m + a.n) * p.pieces + 255) / 256;
-            hipLaunchKernelGGL((matmul_pack_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a, (const T*)x, (const T*)w, (v4i*)workspace, p.pieces);
+            hipLaunchKernelGGL((matmul_pack_kernel<T>), dim3((unsigned)matmul_pack_blocks(p)), dim3(MATMUL_PACK_THREADS), 0, s, a, (const T*)x, (const T*)w, (v4i*)workspace, p.pieces);
             a.a_pitch = a.w_pitch = a.k = 8 * p.pieces;
             xa = workspace, wa = (const v4i*)workspace + (int64_t)a.m * p.pieces;
         }

@@ -41,11 +41,11 @@ typedef struct cldnn_hip_operator_s* cldnn_hip_operator;
 typedef struct {
     int32_t launches;          /* kernels per enqueue */
     int32_t grid, block;       /* of the first of them */
-    int32_t lds_bytes;
+    int32_t lds_bytes;         /* of a workgroup: the most among them */
     int64_t workspace_bytes;   /* device memory that the object holds */
     int64_t ops;               /* floating-point operations of one call */
     int64_t bytes;             /* each input read once, each output written once (attention: of full lengths) */
-    char kernel_name[96];
+    char kernel_name[96];      /* of all of them; products: for operands that are 16-byte aligned, others may take another */
 } cldnn_hip_operator_info;
 
 cldnn_hip_status cldnn_hip_operator_retain(cldnn_hip_operator op);

@@ -151,3 +151,55 @@ def a_recording_outlives_its_operators(kept):
 @pytest.mark.parametrize("kept", [True, False])
 def test_a_recording_holds_the_operators_in_it(on_host, kept):
     on_host(a_recording_outlives_its_operators, kept)
+
+
+READELF = "/opt/rocm/llvm/bin/llvm-readelf"
+
+
+def static_lds(directory):
+    """mangled name -> bytes of LDS that a kernel of the operators' library has by itself"""
+    import re
+
+    import test_mfma_wait_states as scan
+
+    found, hip.LIB_PATH = {}, ops.LIB_PATH
+    for n, image in enumerate(scan.code_objects()):
+        path = os.path.join(directory, "%d.elf" % n)
+        with open(path, "wb") as f:
+            f.write(image)
+        notes = subprocess.run([READELF, "--notes", path], stdout=subprocess.PIPE, check=True, text=True).stdout
+        for kernel in notes.split("  - .agpr_count:")[1:]:
+            value = {k: re.search(r"\.%s:\s+(\S+)" % k, kernel).group(1) for k in ("name", "group_segment_fixed_size")}
+            found[value["name"]] = int(value["group_segment_fixed_size"])
+    return found
+
+
+def infos_describe_the_launches(directory):
+    e = hip.Engine()
+    made = []
+    for b, y, x, f, groups, dtype, out in ((1, 7, 7, 2048, 32, "bf16", "bf16"), (3, 31, 45, 84, 12, "f32", "f16"), (16, 224, 224, 64, 32, "f16", "f16"), (2, 200, 200, 21, 7, "f32", "f32")):
+        made.append((ops.GroupNorm(e, ops.group_norm_desc(ops.map_tensor(dtype, b, y, x, f), groups, out_dtype=out)), 2))
+    for m, n, k in ((4090, 4093, 72), (7160, 2040, 136), (6130, 2046, 64), (3100, 1537, 200), (1601, 1000, 104), (1001, 1000, 264), (190, 2000, 520), (30, 1000, 1000), (7, 250, 9000),
+                    (600, 500, 63), (1601, 1400, 61), (1001, 1000, 255), (3101, 1500, 263), (3101, 1700, 263), (1, 1, 1)):
+        made.append((ops.Matmul(e, ops.matmul_desc(m, n, k, "f16")), 3))
+    for tokens, q, k, size, pairs, pairing in ((196, 16, 16, 64, (16, 16), "halves"), (25088, 16, 4, 128, (16, 24, 24), "interleaved"), (5, 1, 1, 33, (7, 3), "halves_per_axis")):
+        made.append((ops.Rotary(e, ops.rotary_desc(tokens, q, k, size, pairs, "bf16", pairing=pairing)), 5))
+    for b, lq, lk, h, kv, d in ((64, 49, 49, 4, 4, 32), (4, 3136, 3136, 8, 8, 64), (2, 1, 50176, 8, 2, 128), (4, 1030, 130, 4, 4, 104), (2, 1030, 65, 8, 8, 160), (1, 30, 1000, 2, 2, 200)):
+        made.append((ops.Attention(e, ops.attention_desc(b, lq, lk, h, kv, d, "bf16")), 4))
+    lds = static_lds(directory)
+    for op, pointers in made:
+        before = len(launches())
+        op.enqueue(*[AT] * pointers)
+        found, i = launches()[before:], op.info()
+        name = i.kernel_name.decode()
+        assert i.launches == len(found), name
+        assert (i.grid, i.block) == found[0][2:4], "%s: %r, launched %r" % (name, (i.grid, i.block), found[0])
+        assert i.lds_bytes == max(lds[l[1]] + l[4] for l in found), "%s: %d bytes of LDS" % (name, i.lds_bytes)
+        # every kernel is named
+        for part in ("matmul_pack", "matmul_split", "matmul_tile", "matmul_join", "norm_whole", "norm_stats", "norm_apply", "rotary"):
+            assert (part in name) == any(part in l[1] for l in found), "%s: %r" % (name, [l[1] for l in found])
+
+
+@pytest.mark.skipif(not os.path.exists(READELF), reason="needs the kernels' metadata")
+def test_infos_describe_the_launches(on_host, tmp_path):
+    on_host(infos_describe_the_launches, str(tmp_path))
