@@ -220,7 +220,7 @@ class Engine:
     def __init__(self, device=0, profiling=False):
         h = C.c_void_p()
         check(lib().cldnn_hip_engine_create(device, int(profiling), C.byref(h)))
-        self.h = h
+        self.h, self.device = h, device
 
     def info(self):
         i = EngineInfo()

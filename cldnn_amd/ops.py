@@ -2,7 +2,9 @@
 activation and residual, rotary positions, attention.
 
 Only plumbing lives here.  An operator is made once for a shape and enqueued on its engine's stream; what it reads and writes is
-device memory: a hip.Buffer, anything else with a `ptr` or a `data_ptr()`, or an address.  Work of other streams on that memory
+device memory: a hip.Buffer, a torch tensor, anything else with a `ptr` or a `data_ptr()`, or an address.  A tensor has to be on the
+engine's device, of the operand's type (or uint8: plain memory), and either contiguous memory that is large enough, or laid out as the
+operator's description says; a buffer has to be large enough; of an address nothing is known.  Work of other streams on that memory
 has to be ordered by the caller (Engine.finish, events).
 """
 import ctypes as C
@@ -16,6 +18,8 @@ LIB_PATH = os.path.join(os.path.dirname(hip.LIB_PATH), "libcldnn_hip_ops.so")
 
 F32, F16, BF16, I32, NO_TYPE = hip.F32, 4, 5, hip.I32, hip.NO_TYPE
 DT_NAME = {"f32": F32, "f16": F16, "bf16": BF16, "i32": I32}
+TORCH_NAME = {F32: "torch.float32", F16: "torch.float16", BF16: "torch.bfloat16", I32: "torch.int32"}
+SIZE = {F32: 4, F16: 2, BF16: 2, I32: 4}
 POSITION_NAME = {"i32": I32, "f32": F32}
 ACT_NAME = dict(hip.ACT_NAME, silu=4, gelu=5, gelu_tanh=6)
 PAIRING_NAME = {"interleaved": 0, "halves": 1, "halves_per_axis": 2}
@@ -90,10 +94,68 @@ def lib():
     return _lib
 
 
-def _address(x):
-    if x is None or type(x) is int:
-        return x
-    return x.data_ptr() if hasattr(x, "data_ptr") else x.ptr
+class Operand:
+    """What an operator reads or writes at a pointer: elements of `shape`, `strides` elements apart, the first `offset` behind it."""
+
+    def __init__(self, name, dtype, shape, strides, offset=0):
+        self.name, self.dtype, self.shape, self.strides, self.offset = name, dtype, tuple(shape), tuple(strides), offset
+        self.nbytes = (offset + sum((n - 1) * step for n, step in zip(shape, strides)) + 1) * SIZE[dtype]
+
+    @staticmethod
+    def dense(name, dtype, *shape):
+        strides = [1]
+        for n in reversed(shape[1:]):
+            strides.insert(0, strides[0] * n)
+        return Operand(name, dtype, shape, strides)
+
+    def fits(self, t):
+        """a strided tensor as the description has it"""
+        return str(t.dtype) == TORCH_NAME[self.dtype] and tuple(t.shape) == self.shape and not self.offset and all(n == 1 or a == b for n, a, b in zip(self.shape, t.stride(), self.strides))
+
+
+def _check_tensor(t, operand, device):
+    def refuse(what):
+        raise hip.HipError(-2, "%s: %s" % (operand.name, what))
+
+    if t.get_device() != device:
+        refuse("a tensor on %s, not on the engine's device %d" % (t.device, device))
+    if str(t.dtype) not in (TORCH_NAME[operand.dtype], "torch.uint8"):
+        refuse("a tensor of %s" % t.dtype)
+    if not t.is_contiguous() and not operand.fits(t):
+        refuse("a tensor of shape %r and strides %r, described are %r and %r" % (tuple(t.shape), t.stride(), operand.shape, operand.strides))
+    if t.is_contiguous() and t.nbytes < operand.nbytes:
+        refuse("%d bytes, described are %d" % (t.nbytes, operand.nbytes))
+
+
+def _address_of(operand, device):
+    """The function that takes what is given for an operand and returns its address, or refuses it.  operand: None where the description
+    has none, and what is given is not looked at."""
+    if operand is None:
+        return lambda x: None
+    need, kind, dtype = operand.nbytes, None, None  # torch's, once one has come
+
+    def address(x):
+        # what is asked of each tensor is little, in the order of a tensor that fits: 0.2 us beside a launch of 3.5
+        if x.__class__ is kind and x.dtype is dtype and x.get_device() == device and x.nbytes >= need and x.is_contiguous():
+            return x.data_ptr()
+        return checked(x)
+
+    def checked(x):
+        nonlocal kind, dtype
+        if x is None or type(x) is int:
+            return x
+        if hasattr(x, "get_device"):
+            _check_tensor(x, operand, device)
+            if str(x.dtype) == TORCH_NAME[operand.dtype]:
+                kind, dtype = type(x), x.dtype
+            return x.data_ptr()
+        if hasattr(x, "data_ptr"):
+            return x.data_ptr()
+        if getattr(x, "nbytes", need) < need:
+            raise hip.HipError(-2, "%s: a buffer of %d bytes, described are %d" % (operand.name, x.nbytes, need))
+        return x.ptr
+
+    return address
 
 
 def _type(dt):
@@ -159,11 +221,13 @@ def to_type(values, dtype):
 class Operator:
     """What the operators have in common: the object behind the handle."""
 
-    def __init__(self, engine, create, desc):
+    def __init__(self, engine, kind, desc):
         self.engine, self.desc, self.h = engine, desc, None
         h = _P()
-        hip.check(getattr(lib(), create)(engine.h, C.byref(desc), C.byref(h)))
+        hip.check(getattr(lib(), "cldnn_hip_%s_create" % kind)(engine.h, C.byref(desc), C.byref(h)))
         self.h = h
+        self._enqueue = getattr(lib(), "cldnn_hip_%s_enqueue" % kind)
+        self._address = [_address_of(o, engine.device) for o in self._operands(desc)]  # in the entry point's order
 
     def info(self):
         i = OperatorInfo()
@@ -207,11 +271,21 @@ class GroupNorm(Operator):
     """y = act((x - mean) / sqrt(variance + epsilon) * scale + shift), per image and group of features."""
 
     def __init__(self, engine, desc):
-        super().__init__(engine, "cldnn_hip_group_norm_create", desc)
-        self._enqueue = lib().cldnn_hip_group_norm_enqueue
+        super().__init__(engine, "group_norm", desc)
+
+    @staticmethod
+    def _operands(d):
+        def plane(name, t):
+            x = t.pad_lo_f + t.f + t.pad_hi_f
+            y = x * (t.pad_lo_x + t.x + t.pad_hi_x)
+            b = y * (t.pad_lo_y + t.y + t.pad_hi_y)
+            return Operand(name, t.dtype, (t.b, t.y, t.x, t.f), (b, y, x, 1), t.pad_lo_b * b + t.pad_lo_y * y + t.pad_lo_x * x + t.pad_lo_f)
+
+        return plane("input", d.input), Operand.dense("scale", F32, d.input.f), Operand.dense("shift", F32, d.input.f), plane("output", d.output)
 
     def enqueue(self, src, dst, scale=None, shift=None):
-        status = self._enqueue(self.h, _address(src), _address(scale), _address(shift), _address(dst))
+        of_src, of_scale, of_shift, of_dst = self._address
+        status = self._enqueue(self.h, of_src(src), of_scale(scale), of_shift(shift), of_dst(dst))
         if status:
             hip.check(status)
 
@@ -234,11 +308,20 @@ class Matmul(Operator):
     """out = act2(act(a weights^T + bias) + residual)."""
 
     def __init__(self, engine, desc):
-        super().__init__(engine, "cldnn_hip_matmul_create", desc)
-        self._enqueue = lib().cldnn_hip_matmul_enqueue
+        super().__init__(engine, "matmul", desc)
+
+    @staticmethod
+    def _operands(d):
+        def matrix(name, dtype, rows, columns, stride):
+            return Operand(name, dtype, (rows, columns), (stride or columns, 1))
+
+        return (matrix("a", d.dtype, d.m, d.k, d.a_stride), matrix("weights", d.dtype, d.n, d.k, d.weights_stride), Operand.dense("bias", F32, d.n) if d.has_bias else None,
+                matrix("residual", d.residual_dtype, d.m, d.n, d.residual_stride) if d.residual_dtype != NO_TYPE else None,
+                matrix("output", d.out_dtype, d.m, d.n, d.out_stride))
 
     def enqueue(self, a, weights, out, bias=None, residual=None):
-        status = self._enqueue(self.h, _address(a), _address(weights), _address(bias), _address(residual), _address(out))
+        of_a, of_weights, of_bias, of_residual, of_out = self._address
+        status = self._enqueue(self.h, of_a(a), of_weights(weights), of_bias(bias), of_residual(residual), of_out(out))
         if status:
             hip.check(status)
 
@@ -263,11 +346,20 @@ class Rotary(Operator):
     """Queries and keys turned by their tokens' positions along one axis per pair of values."""
 
     def __init__(self, engine, desc):
-        super().__init__(engine, "cldnn_hip_rotary_create", desc)
-        self._enqueue = lib().cldnn_hip_rotary_enqueue
+        super().__init__(engine, "rotary", desc)
+
+    @staticmethod
+    def _operands(d):
+        def heads(name, n, token, head):
+            return Operand(name, d.dtype, (d.tokens, n, d.head_size), (token or n * d.head_size, head or d.head_size, 1)) if n else None
+
+        return (heads("q", d.q_heads, d.q_token_stride, d.q_head_stride), heads("k", d.k_heads, d.k_token_stride, d.k_head_stride),
+                Operand.dense("positions", d.position_dtype, d.tokens, d.axes), heads("q output", d.q_heads, d.q_out_token_stride, d.q_out_head_stride),
+                heads("k output", d.k_heads, d.k_out_token_stride, d.k_out_head_stride))
 
     def enqueue(self, q, k, positions, q_out, k_out):
-        status = self._enqueue(self.h, _address(q), _address(k), _address(positions), _address(q_out), _address(k_out))
+        of_q, of_k, of_positions, of_q_out, of_k_out = self._address
+        status = self._enqueue(self.h, of_q(q), of_k(k), of_positions(positions), of_q_out(q_out), of_k_out(k_out))
         if status:
             hip.check(status)
 
@@ -296,10 +388,24 @@ class Attention(Operator):
     """softmax(scale q k^T + bias) v over the keys below each image's length."""
 
     def __init__(self, engine, desc):
-        super().__init__(engine, "cldnn_hip_attention_create", desc)
-        self._enqueue = lib().cldnn_hip_attention_enqueue
+        super().__init__(engine, "attention", desc)
+
+    @staticmethod
+    def _operands(d):
+        def tokens(name, length, heads, batch, token, head):
+            token = token or heads * d.head_size
+            return Operand(name, d.dtype, (d.batch, length, heads, d.head_size), (batch or length * token, token, head or d.head_size, 1))
+
+        bias = (d.batch, d.q_heads, d.q_len, d.kv_len), (d.bias_batch_stride, d.bias_head_stride, d.bias_q_stride, 1)
+        return (tokens("q", d.q_len, d.q_heads, d.q_batch_stride, d.q_token_stride, d.q_head_stride),
+                tokens("k", d.kv_len, d.kv_heads, d.k_batch_stride, d.k_token_stride, d.k_head_stride),
+                tokens("v", d.kv_len, d.kv_heads, d.v_batch_stride, d.v_token_stride, d.v_head_stride),
+                Operand.dense("key_lengths", I32, d.batch) if d.has_key_lengths else None,
+                Operand("bias", d.bias_dtype, *bias) if d.bias_dtype != NO_TYPE else None,
+                tokens("output", d.q_len, d.q_heads, d.out_batch_stride, d.out_token_stride, d.out_head_stride))
 
     def enqueue(self, q, k, v, out, key_lengths=None, bias=None):
-        status = self._enqueue(self.h, _address(q), _address(k), _address(v), _address(key_lengths), _address(bias), _address(out))
+        of_q, of_k, of_v, of_lengths, of_bias, of_out = self._address
+        status = self._enqueue(self.h, of_q(q), of_k(k), of_v(v), of_lengths(key_lengths), of_bias(bias), of_out(out))
         if status:
             hip.check(status)

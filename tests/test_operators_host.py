@@ -203,3 +203,109 @@ def infos_describe_the_launches(directory):
 @pytest.mark.skipif(not os.path.exists(READELF), reason="needs the kernels' metadata")
 def test_infos_describe_the_launches(on_host, tmp_path):
     on_host(infos_describe_the_launches, str(tmp_path))
+
+
+def a_refusal(call, word):
+    before = len(launches())
+    try:
+        call()
+    except hip.HipError as e:
+        assert e.status == -2 and word in str(e), e
+    else:
+        raise AssertionError("taken: " + word)
+    assert len(launches()) == before
+
+
+def operands_are_checked():
+    import torch
+
+    class OnDevice(torch.Tensor):  # host memory that says it is the device's: nothing reads it
+        def get_device(self):
+            return 0
+
+    def dev(*shape, dtype=torch.float16):
+        return torch.zeros(*shape, dtype=dtype).as_subclass(OnDevice)
+
+    e = hip.Engine()
+    op = ops.Matmul(e, ops.matmul_desc(5, 24, 16, "f16", bias=True, residual=True, out_stride=32))
+    good = dict(a=dev(5, 16), weights=dev(24, 16), out=dev(5, 32), bias=dev(24, dtype=torch.float32), residual=dev(5, 24))
+
+    def call(**other):
+        op.enqueue(**dict(good, **other))
+
+    def taken(**other):
+        before = len(launches())
+        call(**other)
+        assert len(launches()) == before + 1
+
+    taken()
+    # memory, an address, a buffer, a view that is laid out as described
+    taken(a=dev(80), weights=dev(24 * 16 * 2, dtype=torch.uint8), out=dev(5 * 32)[:152], residual=AT)
+    taken(out=dev(5, 32)[:, :24])
+    buffer = ops.Buffer(e, 2 * 5 * 16)
+    taken(a=buffer)
+    a_refusal(lambda: call(a=torch.zeros(5, 16, dtype=torch.float16)), "a: a tensor on cpu")
+    a_refusal(lambda: call(a=dev(16, 5).t()), "a: a tensor of shape (5, 16) and strides (1, 5)")
+    a_refusal(lambda: call(weights=dev(24, 32)[:, :16]), "weights: a tensor of shape (24, 16) and strides (32, 1)")
+    a_refusal(lambda: call(out=dev(5, 32, dtype=torch.uint8)[:, :24]), "output: a tensor of shape")
+    a_refusal(lambda: call(out=dev(5, 24)), "output: 240 bytes, described are 304")
+    a_refusal(lambda: call(residual=dev(5, 24, dtype=torch.bfloat16)), "residual: a tensor of torch.bfloat16")
+    a_refusal(lambda: call(bias=dev(24)), "bias: a tensor of torch.float16")
+    a_refusal(lambda: call(weights=buffer), "weights: a buffer of 160 bytes, described are 768")
+
+    op = ops.Attention(e, ops.attention_desc(2, 3, 70, 4, 2, 32, "bf16", key_lengths=True, bias_shape=(1, 4, 1, 70), k_strides=(70 * 64, 32, 70 * 32)))
+    b16 = torch.bfloat16
+    good = dict(q=dev(2, 3, 4, 32, dtype=b16), k=dev(2, 2, 70, 32, dtype=b16), v=dev(2, 70, 2, 32, dtype=b16), out=dev(2, 3, 4, 32, dtype=b16), key_lengths=dev(2, dtype=torch.int32),
+                bias=dev(1, 4, 1, 70, dtype=b16))
+    taken()
+    taken(k=good["k"].transpose(1, 2))
+    a_refusal(lambda: call(v=good["k"].transpose(1, 2)), "v: a tensor of shape")
+    a_refusal(lambda: call(q=good["q"][:, :2]), "q: a tensor of shape")
+    a_refusal(lambda: call(q=dev(2, 2, 4, 32, dtype=b16)), "q: 1024 bytes, described are 1536")
+    a_refusal(lambda: call(key_lengths=dev(2, dtype=torch.int64)), "key_lengths: a tensor of torch.int64")
+    a_refusal(lambda: call(bias=dev(4, 69, dtype=b16)), "bias: 552 bytes, described are 560")
+
+    op = ops.GroupNorm(e, ops.group_norm_desc(ops.map_tensor("f16", 2, 3, 5, 8, 1, 2, 4), 4, out_dtype="f32"))
+    whole = dev(2, 5, 9, 12)
+    good = dict(src=whole, dst=dev(2, 3, 5, 8, dtype=torch.float32))
+    taken()
+    a_refusal(lambda: call(src=whole[:, 1:4, 2:7, :8]), "input: a tensor of shape")  # the description counts from the padding on
+    a_refusal(lambda: call(dst=dev(2, 3, 5, 8)), "output: a tensor of torch.float16")
+    a_refusal(lambda: call(scale=dev(7, dtype=torch.float32)), "scale: 28 bytes, described are 32")
+
+    op = ops.Rotary(e, ops.rotary_desc(7, 2, 1, 16, (4, 4), "f16", q_strides=(48, 16)))
+    qkv = dev(7, 3, 16)
+    good = dict(q=qkv[:, :2], k=dev(7, 1, 16), positions=dev(7, 2, dtype=torch.int32), q_out=dev(7, 2, 16), k_out=dev(7, 1, 16))
+    taken()
+    taken(q=qkv)
+    a_refusal(lambda: call(k=qkv[:, 2:]), "k: a tensor of shape")
+    a_refusal(lambda: call(positions=dev(7, 2, dtype=torch.float32)), "positions: a tensor of torch.float32")
+
+
+def test_operands_are_checked(on_host):
+    on_host(operands_are_checked)
+
+
+def entry_points_refuse():
+    """the C entry points themselves, given addresses"""
+    e = hip.Engine()
+    made = [  # operator, how many pointers, the alignment of each in bytes, those that may be null
+        (ops.GroupNorm(e, ops.group_norm_desc(ops.map_tensor("f16", 1, 4, 4, 12), 4, out_dtype="f32")), (2, 4, 4, 4), (1, 2)),
+        (ops.Matmul(e, ops.matmul_desc(4, 4, 4, "f16", bias=True, residual=True, residual_dtype="f32")), (2, 2, 4, 4, 2), ()),
+        (ops.Matmul(e, ops.matmul_desc(4, 4, 4, "f16", out_dtype="f32")), (2, 2, 1, 1, 4), (2, 3)),
+        (ops.Rotary(e, ops.rotary_desc(4, 2, 2, 16, (4, 4), "f16")), (2, 2, 4, 2, 2), ()),
+        (ops.Attention(e, ops.attention_desc(1, 4, 4, 2, 2, 32, "f16", key_lengths=True, bias_shape=(1, 1, 4, 4))), (16, 16, 16, 4, 2, 16), ()),
+    ]
+    for op, aligned, optional in made:
+        assert op._enqueue(op.h, *[AT] * len(aligned)) == 0
+        for i, to in enumerate(aligned):
+            pointers = [AT] * len(aligned)
+            pointers[i] = None
+            assert (op._enqueue(op.h, *pointers) == 0) == (i in optional), (type(op), i)
+            if to > 1:
+                pointers[i] = AT + to // 2
+                assert op._enqueue(op.h, *pointers) == -2 and b"aligned" in hip.lib().cldnn_hip_last_error(), (type(op), i)
+
+
+def test_entry_points_refuse(on_host):
+    on_host(entry_points_refuse)
