@@ -382,7 +382,7 @@ AttentionPlan* attention_plan(const cldnn_hip_engine_s& e, const cldnn_hip_atten
     // other.  (us, parts of 2, 4, 8 tiles: 1 query, 4096 keys, 8 key heads of 128: 12.6, 15.4, 22.3; all in one: 115.  5 tiles: 10.7 in
     // two parts, 9.4 in one.  2 x 2 key heads over 50176 keys: 28.9 with two workgroups to a CU, 32.5 and 36.2 with one and four)
     if (few && tiles >= 6) a.splits = (int)std::max<int64_t>(1, std::min<int64_t>((2 * cus + a.blocks * pairs - 1) / (a.blocks * pairs), std::min(tiles / 2, ATT_MOST_SPLITS)));
-    CHIP_REQUIRE(a.blocks * pairs * a.splits < (1ll << 31), CLDNN_HIP_UNSUPPORTED_SIZE, "attention: too large");
+    check_grid(a.blocks * pairs * a.splits, 64 * plan->waves, "attention");
     a.total = (int)(a.blocks * pairs * a.splits);
     const int64_t scores = (int64_t)d.batch * d.q_heads * d.q_len * d.kv_len;
     const int64_t bias_size = d.bias_dtype == CLDNN_HIP_NO_TYPE ? 0 : d.bias_dtype == CLDNN_HIP_F32 ? 4 : 2;

@@ -452,7 +452,7 @@ static int matmul_choose(int m, int n, bool whole, int cus)
 static void matmul_tiles(MatmulArgs& a, const MatmulKernel& k)
 {
     const int64_t tiles = matmul_count(a.m, a.n, k);
-    CHIP_REQUIRE(tiles < (1ll << 31), CLDNN_HIP_UNSUPPORTED_SIZE, "matmul: too large");
+    check_grid(tiles, 64 * k.waves, "matmul");
     a.tiles = (int32_t)tiles, a.tiles_m = (a.m + k.rows - 1) / k.rows, a.tiles_n = (a.n + k.features - 1) / k.features;
     a.band = 8;
 }
@@ -461,6 +461,8 @@ MatmulPlan* matmul_plan(const cldnn_hip_engine_s& e, const cldnn_hip_matmul_desc
 {
     const auto is_half = [](int dt) { return dt == CLDNN_HIP_F16 || dt == CLDNN_HIP_BF16; };
     CHIP_REQUIRE(d.m > 0 && d.n > 0 && d.k > 0, CLDNN_HIP_INVALID_ARG, "matmul: sizes must be positive");
+    // so that a tile's last row or feature, and a step's last value, has a number
+    CHIP_REQUIRE(std::max(d.m, std::max(d.n, d.k)) <= INT32_MAX - 256, CLDNN_HIP_UNSUPPORTED_SIZE, "matmul: too large");
     CHIP_REQUIRE(is_half(d.dtype), CLDNN_HIP_INVALID_ARG, "matmul: a and weights must be f16 or bf16");
     CHIP_REQUIRE(d.out_dtype == d.dtype || d.out_dtype == CLDNN_HIP_F32, CLDNN_HIP_INVALID_ARG, "matmul: the output must be of a's type or f32");
     CHIP_REQUIRE(d.residual_dtype == d.dtype || d.residual_dtype == CLDNN_HIP_F32 || d.residual_dtype == CLDNN_HIP_NO_TYPE, CLDNN_HIP_INVALID_ARG,
@@ -489,7 +491,7 @@ MatmulPlan* matmul_plan(const cldnn_hip_engine_s& e, const cldnn_hip_matmul_desc
     plan->any = matmul_choose(d.m, d.n, false, cus);
     // The copy costs a launch and two trips of the operands, the kernels for any rows 5 times the tiles' time from there on (4000 x 255
     // -> 1000: 41 us without it, 10 with).
-    if (!whole && plan->any != MM_16 && d.k < (1 << 20) && (double)d.m * d.n * d.k >= MATMUL_PACK && ((int64_t)d.m + d.n) * ((d.k + 7) / 8) < (1ll << 38)) {
+    if (!whole && plan->any != MM_16 && d.k < (1 << 20) && (double)d.m * d.n * d.k >= MATMUL_PACK && ((int64_t)d.m + d.n) * ((d.k + 7) / 8) < (1ll << 32) - MATMUL_PACK_THREADS) {
         plan->pieces = (d.k + 7) / 8;
         plan->kernel = matmul_choose(d.m, d.n, true, cus);
     }

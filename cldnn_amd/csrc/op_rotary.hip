@@ -168,8 +168,10 @@ RotaryPlan* rotary_plan(const cldnn_hip_engine_s& e, const cldnn_hip_rotary_desc
     };
     while (!fits(plan->width)) plan->width /= 2;
     a.items = a.pairs / plan->width + (a.copied + 7) / 8;
+    CHIP_REQUIRE(d.tokens < (1ll << 32), CLDNN_HIP_UNSUPPORTED_SIZE, "rotary: too many tokens");
     const int64_t blocks = (d.tokens * a.items + ROTARY_THREADS - 1) / ROTARY_THREADS;
-    CHIP_REQUIRE(d.tokens < (1ll << 40) && blocks < (1ll << 31), CLDNN_HIP_UNSUPPORTED_SIZE, "rotary: too many tokens");
+    check_grid(blocks, ROTARY_THREADS, "rotary");
+    CHIP_REQUIRE(std::max(d.q_heads, d.k_heads) < (1 << 29), CLDNN_HIP_UNSUPPORTED_SIZE, "rotary: too many heads");
     // heads in groups where threads are few: four waves to a SIMD before a thread takes a second group of four
     const int heads = d.q_heads + d.k_heads;
     const int64_t wanted = std::max<int64_t>(1, 4ll * e.props.multiProcessorCount / blocks);

@@ -186,6 +186,12 @@ inline void check_aligned(const void* p, size_t to, const char* what)
     CHIP_REQUIRE(((uintptr_t)p & (to - 1)) == 0, CLDNN_HIP_INVALID_ARG, std::string(what) + " is not aligned to " + std::to_string(to) + " bytes");
 }
 
+// the runtime counts a grid's threads along an axis in 32 bits
+inline void check_grid(int64_t blocks, int threads, const char* what)
+{
+    CHIP_REQUIRE(blocks < (1ll << 32) / threads, CLDNN_HIP_UNSUPPORTED_SIZE, std::string(what) + ": too large");
+}
+
 inline Act make_act(int32_t kind, float m, float n, const char* what)
 {
     CHIP_REQUIRE(kind >= CLDNN_HIP_ACT_NONE && kind <= CLDNN_HIP_ACT_GELU_TANH, CLDNN_HIP_INVALID_ARG, std::string(what) + ": unknown activation");

@@ -309,3 +309,39 @@ def entry_points_refuse():
 
 def test_entry_points_refuse(on_host):
     on_host(entry_points_refuse)
+
+
+def grids_hold_what_they_launch():
+    """The runtime counts the threads of a grid in 32 bits, and the kernels rows and features in 31: a size beyond is refused when the
+    object is made, whatever memory there is."""
+    e = hip.Engine()
+    most = (1 << 31) - 1
+
+    def status(kind, desc):
+        try:
+            kind(e, desc).close()
+            return 0
+        except hip.HipError as x:
+            assert "too" in str(x), x
+            return x.status
+
+    for m, n, k in ((most, 8, 8), (most - 200, 8, 8), (8, most, 8), (most, 1, 1), (1, most, 3), (1, 1, most), (2, 2, most - 8), (most - 300, 1 << 17, 8), (1 << 30, 1 << 13, 9)):
+        assert status(ops.Matmul, ops.matmul_desc(m, n, k, "f16")) == -5, (m, n, k)
+    for size in ((65535, 1, 1, 512, 512, 32), (65535, 300, 300, 128, 128, 64)):
+        assert status(ops.Attention, ops.attention_desc(*size, "f16")) == -5, size
+    for tokens, heads in ((1 << 30, 1), (1 << 41, 1), (4, most)):
+        assert status(ops.Rotary, ops.rotary_desc(tokens, heads, heads if heads > 1 else 0, 64, (32,), "f32")) == -5, (tokens, heads)
+    # the largest that are left
+    made = [(ops.Matmul(e, ops.matmul_desc(m, n, k, "f16")), 3, -(-m // rows) * -(-n // columns)) for m, n, k, rows, columns in (
+        (1 << 30, 64, 8, 128, 128), (1 << 28, 8, 129, 64, 64), (1, (1 << 30) - 7, 8, 128, 128), (7, 3, most - 300, 16, 16))]
+    made += [(ops.Rotary(e, ops.rotary_desc((1 << 28) - 1, 1, 0, 64, (32,), "f16")), 5, -(-((1 << 28) - 1) * 8 // 256))]
+    made += [(ops.Attention(e, ops.attention_desc(65535, 1, 1, 255, 255, 32, "f16")), 4, 65535 * 255)]
+    for op, pointers, workgroups in made:
+        before = len(launches())
+        op.enqueue(*[AT] * pointers)
+        grid = launches()[before][2:4]
+        assert grid[0] % workgroups == 0 and grid[0] * grid[1] < 1 << 32, (op.info().kernel_name, grid, workgroups)
+
+
+def test_grids_hold_what_they_launch(on_host):
+    on_host(grids_hold_what_they_launch)
