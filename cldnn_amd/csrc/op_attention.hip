@@ -15,6 +15,8 @@
 //
 // The waves of a workgroup share tiles of 64 keys, which direct loads bring into LDS one tile ahead.  Where rows are few the keys
 // are split over workgroups (of one wave then), and a second kernel joins their parts.
+#include <cfloat>
+
 #include "ops_common.h"
 
 namespace chip {
@@ -37,6 +39,7 @@ struct AttentionPlan {
 };
 
 constexpr int ATT_KEYS = 64;  // of a tile
+constexpr float ATT_LARGE = 4096.0f;  // powers of two from which on a score's product with its unit is not good to 12 bits behind the point
 constexpr int ATT_ONE_WAVE = 128;  // largest head that a workgroup of one wave is made for: beyond, a CU holds one tile anyway
 
 // Piece c (16 bytes) of row r of D values lies at place r * D / 8 + (c ^ att_turn(r)) of a tile in LDS: sixteen neighbouring rows
@@ -159,6 +162,8 @@ __global__ __launch_bounds__(64 * WAVES, D <= 64 ? (std::is_same<B, void>::value
 
     v16f o[BLOCKS] = {};
     float most = -INFINITY, sum = 0.0f;
+    float base = 0.0f, under = 0.0f;  // the maximum, and its product with the unit, that the exponents are taken from
+    bool large = false;
     if (first < last) load(first, 0);
     for (int tile = first, at = 0; tile < last; ++tile, at ^= 1) {
         if constexpr (FAR) __syncthreads();
@@ -203,7 +208,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 64 ? (std::is_same<B, void>::value
         top = att_both(top, [](float x, float y) { return fmaxf(x, y); });
         // The maximum that the exponents are taken from follows when it is left behind by 2^8, which the sums and the operands of the
         // second product hold without loss: after the first tiles hardly ever.
-        if (__any(top > most + a.margin)) {
+        if (__any(top > most + a.margin) || large) {
             const bool follow = top > most + a.margin;
             const float fade = follow ? __builtin_amdgcn_exp2f((most - top) * a.unit) : 1.0f;
             most = follow ? top : most;
@@ -212,9 +217,21 @@ __global__ __launch_bounds__(64 * WAVES, D <= 64 ? (std::is_same<B, void>::value
             for (int i = 0; i < BLOCKS; ++i)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) o[i][j] *= fade;
+            base = most == -INFINITY ? 0.0f : most;  // a row without a key so far
+            if constexpr (!BIAS) {
+                // The rounding of a large product with the unit would show in the exponents, where it no longer is that of the scores
+                // alone: they are taken from the maximum first then.
+                under = base * a.unit;
+                large = __any(__builtin_fabsf(under) > ATT_LARGE);
+                if (large) {
+                    under = 0.0f;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[t][i] -= base;
+                }
+            }
         }
-        const float base = most == -INFINITY ? 0.0f : most;  // a row without a key so far
-        const float under = base * a.unit;
         V8 p[4];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -350,7 +367,8 @@ AttentionPlan* attention_plan(const cldnn_hip_engine_s& e, const cldnn_hip_atten
     a.negative = scale < 0.0f;
     a.scale = std::fabs(scale);
     a.unit = 1.44269504f * (d.bias_dtype == CLDNN_HIP_NO_TYPE ? a.scale : 1.0f);
-    a.margin = 8.0f / a.unit;
+    CHIP_REQUIRE(std::isfinite(a.unit), CLDNN_HIP_INVALID_ARG, "attention: a scale too large for 32 bits");
+    a.margin = std::min(8.0f / a.unit, FLT_MAX);  // minus infinity stays below every score
     const auto strides = [&](int heads, int len, int64_t batch, int64_t token, int64_t head, int64_t& pb, int64_t& pt, int64_t& ph) {
         ph = head ? head : d.head_size;
         pt = token ? token : (int64_t)heads * d.head_size;

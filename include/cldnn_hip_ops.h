@@ -136,7 +136,7 @@ cldnn_hip_status cldnn_hip_rotary_enqueue(cldnn_hip_operator op, const void* q_d
 typedef struct {
     int32_t batch, q_len, kv_len, q_heads, kv_heads, head_size;  /* q_heads a multiple of kv_heads */
     int32_t dtype;
-    float scale;                      /* 0 = 1 / sqrt(head_size) */
+    float scale;                      /* 0 = 1 / sqrt(head_size); log2(e) times it has to be finite */
     int32_t has_key_lengths;
     int32_t bias_dtype;               /* dtype, CLDNN_HIP_F32, or CLDNN_HIP_NO_TYPE: none */
     /* elements; 0 = dense [batch][len][heads][head_size] */

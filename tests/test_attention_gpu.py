@@ -158,6 +158,34 @@ def test_scales_and_sharp_rows(eng, scale, lq):
     check(eng, 1, lq, 300, 2, 2, 64, "f16", scale=scale, spread=2.0)
 
 
+@pytest.mark.parametrize("scale", [1e-39, -1e-44, 3e-38, 1e30])
+@pytest.mark.parametrize("size", [(1, 40, 300, 2, 2), (1, 1, 2000, 2, 2), (2, 1, 3, 2, 1)], ids=str)
+def test_scales_at_the_ends_of_their_range(eng, scale, size):
+    # next to nothing: the mean of the values; next to infinite: the value of the largest score
+    b, lq, lk, h, kv = size
+    g = generator(12)
+    q, k, v = (random(g, b, n, heads, 64, dtype="f16") for n, heads in ((lq, h), (lk, kv), (lk, kv)))
+    out = torch.empty(b, lq, h, 64, dtype=torch.float16, device="cuda")
+    op = ops.Attention(eng, ops.attention_desc(b, lq, lk, h, kv, 64, "f16", scale=scale))
+    run(eng, op, q.cuda(), k.cuda(), v.cuda(), out)
+    op.close()
+    for i in range(b):
+        for j in range(h):
+            vd = v[i, :, j * kv // h].double()
+            if abs(scale) < 1:
+                want, size = vd.mean(0).expand(lq, 64), vd.abs().mean(0)
+            else:
+                want = vd[(q[i, :, j].double() @ k[i, :, j * kv // h].double().T).argmax(1)]
+                size = want.abs()
+            close(out[i, :, j], want, 2 * HALF_ULP["f16"] * size + (lk + 8) * EPS * size + SMALLEST["f16"], "scale %g" % scale)
+
+
+def test_scales_that_32_bits_cannot_turn_into_powers_of_two(eng):
+    assert refused(eng, ops.Attention, ops.attention_desc(1, 4, 4, 2, 2, 32, "f16", scale=3e38)) == INVALID_ARG
+    assert refused(eng, ops.Attention, ops.attention_desc(1, 4, 4, 2, 2, 32, "f16", scale=-3e38)) == INVALID_ARG
+    assert refused(eng, ops.Attention, ops.attention_desc(1, 4, 4, 2, 2, 32, "f16", scale=3e38, bias_shape=(1, 1, 4, 4))) == 0
+
+
 @pytest.mark.parametrize("lq", [33, 1])
 def test_nan_and_infinity_within_the_lengths_count(eng, lq):
     g = generator(8)
