@@ -1,8 +1,10 @@
 // Group norm with an activation, channels last.
 //
-// Per image and group: mean and M2 = sum (x - mean)^2 over the group's features and the whole plane.  A thread sums its own few
-// pixels of a feature around the first of them, K: with s1 = sum (x - K), s2 = sum (x - K)^2 over n values, mean = K + s1 / n and
-// M2 = s2 - s1^2 / n, where K being one of the values bounds s2 / M2 by n (a K shared by a workgroup's rows made that hundreds).
+// Per image and group: mean and M2 = sum (x - mean)^2 over the group's features and the whole plane.  A thread sums its own
+// pixels of a feature around a value K, the mean of its c first ones: with s1 = sum (x - K), s2 = sum (x - K)^2 over the others, n
+// values in all have mean = K + s1 / n and M2 = M2 of the c + s2 - s1^2 / n.  s2 is at most n / c of the result then, which is
+// what its rounding grows by; K is the first value, and moved to the mean after 8, 64 .. others, so that n / c stays below 10.  (With
+// the first value all the way, one unlike the rest cost 4e-3 of M2 at 1600 pixels to a thread, and costs 2e-6 so.)
 // Parts are joined by M2 = sum M2_i + sum n_i (mean_i - mean)^2 (Chan, Golub and LeVeque), in an order that the shapes alone fix.
 #include "ops_common.h"
 
@@ -81,11 +83,22 @@ __device__ inline int norm_share(int n, int r, int rows) { return (n - r + rows 
 // mean and M2 of values a vector holds
 template <int V>
 struct NormSums {
-    float K[V], s1[V], s2[V];
+    float K[V], s1[V], s2[V], M2[V];
     __device__ void start(const float (&v)[V])
     {
 #pragma unroll
-        for (int i = 0; i < V; ++i) K[i] = v[i], s1[i] = s2[i] = 0.0f;
+        for (int i = 0; i < V; ++i) K[i] = v[i], s1[i] = s2[i] = M2[i] = 0.0f;
+    }
+    // K becomes the mean of the n values so far
+    __device__ void move(int n)
+    {
+        const float own = 1.0f / (float)n;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float m = s1[i] * own;
+            K[i] += m, M2[i] += s2[i] - s1[i] * m;
+            s1[i] = s2[i] = 0.0f;
+        }
     }
     __device__ void add(const float (&v)[V])
     {
@@ -97,15 +110,10 @@ struct NormSums {
         }
     }
     // neighbours of one group, 2^fold of them, are one part: parts of n values each are joined two by two
-    __device__ void put(const NormArgs& a, float2* row, int c, int n) const
+    __device__ void put(const NormArgs& a, float2* row, int c, int n)
     {
-        const float own = 1.0f / (float)n;
-        float mean[V], M2[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float m = s1[i] * own;
-            mean[i] = K[i] + m, M2[i] = s2[i] - s1[i] * m;
-        }
+        move(n);
+        float (&mean)[V] = K;
         float half = 0.5f * (float)n;
 #pragma unroll
         for (int step = 1; step < V; step *= 2) {
@@ -200,10 +208,16 @@ __device__ inline void norm_sum(const NormArgs& a, const TI* src, int span, int 
         float v[V];
         norm_load<TI, V>(src + c + norm_pixel(a, a.in_py, a.in_px, p0 + r), v);
         sums.start(v);
+        int p = r + a.rows, so_far = 1;
+        for (int more = 8; p < n; more *= 8) {
+            const int end = (int)min((int64_t)n, p + (int64_t)more * a.rows);
 #pragma unroll 4
-        for (int p = r + a.rows; p < n; p += a.rows) {
-            norm_load<TI, V>(src + c + norm_pixel(a, a.in_py, a.in_px, p0 + p), v);
-            sums.add(v);
+            for (; p < end; p += a.rows) {
+                norm_load<TI, V>(src + c + norm_pixel(a, a.in_py, a.in_px, p0 + p), v);
+                sums.add(v);
+            }
+            so_far += more;
+            if (p < n) sums.move(so_far);
         }
         sums.put(a, rows + r * (a.span >> a.fold), c, norm_share(n, r, a.rows));
     }
@@ -262,7 +276,7 @@ __device__ inline void norm_finish(const NormArgs& a, const TI* src, TO* dst, in
 }
 
 // A plane to a workgroup: the second reading finds it in the caches.  One launch.  (7x7x2048, one image: 6.2 us, of it 4.3 the launch,
-// the rest three trips to memory and the join; 32 of 56x56x256, f16: 32 us, 3.2 TB/s of one reading and one writing.  The plane held in
+// the rest three trips to memory and the join; 32 of 56x56x256, f16: 33 us, 3.1 TB/s of one reading and one writing.  The plane held in
 // registers instead takes the same time and more program.)
 template <typename TI, typename TO, int V>
 __global__ __launch_bounds__(NORM_MOST_THREADS) void norm_whole_kernel(NormArgs a, const TI* in, const float* scale, const float* shift, TO* out)

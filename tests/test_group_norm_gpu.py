@@ -140,6 +140,29 @@ def test_offsets_past_32_bits(eng):
     close(dst.view(y * x, 1 << 26)[:, :f].reshape(1, y, x, f), want, bound + HALF_ULP["bf16"] * want.abs() * (1 + 2 ** -8))
 
 
+@pytest.mark.parametrize("first", ["one", "rows"])
+@pytest.mark.parametrize("batch,y,x,f,groups,dtype,spare", [(256, 40, 50, 1023, 31, "f32", 0), (256, 41, 35, 1023, 31, "f16", 1), (64, 40, 40, 8192, 256, "f16", 0)])
+def test_first_pixels_unlike_the_rest_of_many(eng, batch, y, x, f, groups, dtype, spare, first):
+    """hundreds of pixels to a thread, the first (or the first rows) far from all others: a border, a corner"""
+    g = torch.Generator("cuda")
+    g.manual_seed(batch + f)
+    data = torch.empty(batch, y, x, f + spare, dtype=TYPES[dtype], device="cuda")
+    for image in data:
+        image.copy_(10 + 0.1 * torch.randn(y, x, f + spare, generator=g, device="cuda"))
+    if first == "one":
+        data[:, 0, 0] = 0
+    else:
+        data[:, :2] = 0
+    t = ops.map_tensor(dtype, batch, y, x, f, pad_f=spare)
+    op = ops.GroupNorm(eng, ops.group_norm_desc(t, groups, out_dtype="f32"))
+    out = torch.empty(batch, y, x, f, device="cuda")
+    run(eng, op, data, out)
+    op.close()
+    for i in (0, batch - 1):
+        v, want, bound = reference(data[i:i + 1, :, :, :f].cpu(), groups, None, None, 1e-5, "none", 0, 0)
+        close(out[i:i + 1], want, bound + HALF_ULP["f32"] * want.abs())
+
+
 def test_nan_and_infinity_stay_in_their_group(eng):
     g = generator(13)
     data = random(g, 2, 5, 5, 32)
