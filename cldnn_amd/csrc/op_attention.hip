@@ -86,8 +86,11 @@ __device__ inline float att_add(__bf16 a, __bf16 b, float sum)
 }
 __device__ inline float att_add(_Float16 a, _Float16 b, float sum) { return sum + (float)a + (float)b; }
 
+// Waves to a SIMD: what the registers of four and eight waves sharing a tile leave.  A workgroup of one wave has a tile of its own, and
+// LDS holds two to ten of those to a CU (D 128 to 32).  Of all, heads up to 160 with an f32 bias and up to 256 with keys that are far
+// apart and a bias run out of registers, by 3 to 26 that lie in scratch memory.
 template <typename T, int D, typename B, int WAVES, bool FAR>
-__global__ __launch_bounds__(64 * WAVES, D <= 64 ? (std::is_same<B, void>::value ? 4 : 3) : D <= 160 ? 2 : 1) void attention_kernel(AttentionArgs a, const T* q, const T* k, const T* v, const int32_t* lengths, const B* bias, T* out, float* part)
+__global__ __launch_bounds__(64 * WAVES, WAVES == 1 ? (D <= 32 ? 3 : 1) : D <= 64 ? (std::is_same<B, void>::value ? 4 : 3) : D <= 160 ? 2 : 1) void attention_kernel(AttentionArgs a, const T* q, const T* k, const T* v, const int32_t* lengths, const B* bias, T* out, float* part)
 {
     typedef typename vec8<T>::type V8;
     constexpr int C = D / 8, STEPS = D / 16, BLOCKS = D / 32, TILE = ATT_KEYS * C, LOADS = C / WAVES;

@@ -252,7 +252,7 @@ __global__ __launch_bounds__(256) void matmul_join_kernel(MatmulArgs a, void* ou
 // Row 16 t + r of a wave's 64 rows of weights is feature 16 (r / 4) + 4 t + r % 4 of its 64: the four results that the matrix
 // instruction leaves in a lane are neighbours, and so are those of the four blocks t: 16 features of one row of the result.
 template <typename T, int WM, int WN, int MB, int ST, int KG>
-__global__ __launch_bounds__(64 * WM * WN * KG, KG > 2 ? KG : 2) void matmul_tile_kernel(MatmulArgs a, const T* x, const T* w, void* out)
+__global__ __launch_bounds__(64 * WM * WN * KG, 2) void matmul_tile_kernel(MatmulArgs a, const T* x, const T* w, void* out)
 {
     typedef typename vec8<T>::type V;
     constexpr int WAVES = WM * WN, BM = WM * MB * 16, BN = WN * 64, BK = 64;
