@@ -34,6 +34,7 @@ struct NormPlan {
 };
 
 constexpr int NORM_MOST_SPAN = 6144;  // features of a workgroup: their sums lie in LDS
+// Leaves 128 registers to a thread: with vectors of 8, norm_apply keeps 9 to 14 values in scratch memory and norm_whole 50 to 60.
 constexpr int NORM_MOST_THREADS = 1024;
 // Vectors of a plane up to which one workgroup takes it (us, one launch and two: 32 of 56x56x256 f16, 12544 vectors, 33 and 54; one
 // of 64x64x320, 20480 vectors, 33 and 15).
@@ -429,7 +430,9 @@ void norm_launch(hipStream_t s, const NormPlan& p, void* workspace, const void* 
     with_float(p.in_dt, [&](auto ti) {
         with_float(p.out_dt, [&](auto to) {
             switch (p.vec) {
-            case 8: both(ti, to, std::integral_constant<int, 8>()); break;
+            case 8:
+                if constexpr (sizeof(ti) == 2) both(ti, to, std::integral_constant<int, 8>());
+                break;
             case 4: both(ti, to, std::integral_constant<int, 4>()); break;
             case 2: both(ti, to, std::integral_constant<int, 2>()); break;
             default: both(ti, to, std::integral_constant<int, 1>());

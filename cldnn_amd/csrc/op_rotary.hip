@@ -198,8 +198,12 @@ void rotary_launch(hipStream_t s, const RotaryPlan& p, const void* workspace, co
         typedef decltype(t) T;
         const auto launch = [&](auto w) {
             constexpr int W = decltype(w)::value;
-            const auto f = a.interleaved ? rotary_kernel<T, W <= 4 ? W : 1, true> : rotary_kernel<T, W, false>;
-            hipLaunchKernelGGL(f, grid, dim3(ROTARY_THREADS), 0, s, a, (const RotaryPair*)workspace, positions, (const T*)q, (const T*)k, (T*)q_out, (T*)k_out);
+            const auto go = [&](auto f) {
+                hipLaunchKernelGGL(f, grid, dim3(ROTARY_THREADS), 0, s, a, (const RotaryPair*)workspace, positions, (const T*)q, (const T*)k, (T*)q_out, (T*)k_out);
+            };
+            if (!a.interleaved) {
+                if constexpr (W * sizeof(T) <= 16) go(rotary_kernel<T, W, false>);
+            } else if constexpr (2 * W * sizeof(T) <= 16) go(rotary_kernel<T, W, true>);
         };
         switch (p.width) {
         case 8: launch(std::integral_constant<int, 8>()); break;
