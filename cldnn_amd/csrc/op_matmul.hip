@@ -132,9 +132,10 @@ __device__ inline void matmul_meet()
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// Few rows, or few tiles: 16 FT features x 16 PT rows to a workgroup, whose waves split K; both operands straight from memory into
-// the registers that the matrix instruction reads, U steps of 32 at a time; the partial sums meet in LDS.  Bound by the weights: 1 x
-// 25088 -> 4096 39 us, 5.3 TB/s, a large copy's rate; with 16 rows 55 us, their values being as many bytes again from the die's L2.
+// Few rows, or few tiles: 16 FT features x 16 PT rows to a workgroup, whose waves split K in runs of U steps of 32; both operands
+// straight from memory into the registers that the matrix instruction reads; the partial sums meet in LDS.  Of a run of 16 steps the
+// compiler keeps twelve loads, six steps, under way (70 registers) and lets them run out at its end.  Bound by the weights: 1 x 25088
+// -> 4096 39 us, 5.3 TB/s, a large copy's rate; with 16 rows 55 us, their values being as many bytes again from the die's L2.
 template <typename T, int FT, int PT, int U, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void matmul_split_kernel(MatmulArgs a, const T* x, const T* w, void* out)
 {
@@ -432,7 +433,8 @@ static int matmul_choose(int m, int n, bool whole, int cus)
     const auto tiles = [&](int row) { return matmul_count(m, n, matmul_kernels[row]); };
     const auto rounds = [&](int row) { return (tiles(row) + cus - 1) / cus; };
     // Few tiles of any size: the smallest, whose eight waves split K.  (us, against 32 x 64 tiles: 1 x 2048 -> 1000 4.7 and 7.0, 64 x 2048
-    // -> 1000 6.0 and 7.0; at twice as many tiles, 32 x 1024 -> 4096, 6.0 and 5.2)
+    // -> 1000 6.0 and 7.0; at twice as many tiles, 32 x 1024 -> 4096, 6.0 and 5.2.  The bound is that of such K; at 8192 it is late: 16 x
+    // 8192 -> 5120, 320 of them, 30.7, -> 5136 in 32 x 64 tiles 17.6)
     if (tiles(MM_16) * 4 <= cus * 5) return MM_16;
     if (!whole) return tiles(MM_ANY_64) >= cus ? MM_ANY_64 : MM_ANY_32;
     if (tiles(MM_128) * 4 >= cus * 5) {
@@ -499,7 +501,8 @@ MatmulPlan* matmul_plan(const cldnn_hip_engine_s& e, const cldnn_hip_matmul_desc
     matmul_tiles(a, kernel);
     // The smallest tiles that leave half of the chip idle over a long K: several workgroups to a tile, for the price of a second launch.
     // Without it and with it: 16 x 1000 x 25088 44.9 and 20.3 us, 1 x 500 x 25088 29.0 and 10.8, 8 x 1000 x 16384 24.9 and 12.4,
-    // 4 x 2000 x 8000 12.5 and 11.6; 1 x 1000 x 4096 6.6 and 9.3, so from 8000 on.
+    // 4 x 2000 x 8000 12.5 and 11.6; 1 x 1000 x 4096 6.6 and 9.3, so from 8000 on.  Beyond half of the chip it is not done, and the step
+    // shows: 16 x 2048 x 25088, 128 tiles of two workgroups, 31.4 us, 16 x 2064 x 25088, 129 of one, 50.8.
     a.splits = 1;
     if (plan->kernel == MM_16 && a.tiles * 2 <= cus && d.k >= 8000) a.splits = std::min(cus / a.tiles, d.k / 2048);
     info.launches = plan->pieces || a.splits > 1 ? 2 : 1, info.block = 64 * kernel.waves, info.grid = a.tiles * a.splits, info.lds_bytes = kernel.lds;
