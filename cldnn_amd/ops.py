@@ -3,7 +3,7 @@ activation and residual, rotary positions, attention.
 
 Only plumbing lives here.  An operator is made once for a shape and enqueued on its engine's stream; what it reads and writes is
 device memory: a hip.Buffer, a torch tensor, anything else with a `ptr` or a `data_ptr()`, or an address.  A tensor has to be on the
-engine's device, of the operand's type (or uint8: plain memory), and either contiguous memory that is large enough, or laid out as the
+engine's device or in pinned memory, of the operand's type (or uint8: plain memory), and either contiguous memory that is large enough, or laid out as the
 operator's description says; a buffer has to be large enough; of an address nothing is known.  Work of other streams on that memory
 has to be ordered by the caller (Engine.finish, events).
 """
@@ -117,7 +117,7 @@ def _check_tensor(t, operand, device):
     def refuse(what):
         raise hip.HipError(-2, "%s: %s" % (operand.name, what))
 
-    if t.get_device() != device:
+    if t.get_device() != device and not (t.device.type == "cpu" and t.is_pinned()):
         refuse("a tensor on %s, not on the engine's device %d" % (t.device, device))
     if str(t.dtype) not in (TORCH_NAME[operand.dtype], "torch.uint8"):
         refuse("a tensor of %s" % t.dtype)

@@ -1,4 +1,5 @@
-"""One operator of two kernels, enqueued by two threads with data of their own: each result is that of the call alone."""
+"""One operator of two kernels, enqueued by two threads with data of their own: each result is that of the call alone.  A recording
+that outlives its operator.  Operands in pinned host memory."""
 import threading
 
 import pytest
@@ -56,4 +57,48 @@ def test_threads_that_enqueue_one_operator(eng, name):
     eng.finish()
     for n in range(2):
         assert all(torch.equal(y, want[n]) for y in got[n])
+    op.close()
+
+
+@pytest.mark.parametrize("name", ["norm", "packed", "joined", "attention"])
+def test_a_recording_outlives_its_operator(eng, name):
+    op, inner, outer, call = operators(eng)[name]
+    x = random(generator(7), *inner, dtype="f16").cuda()
+    want, got = (torch.zeros(outer, dtype=torch.float16, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    call(op, x, want)
+    L, rec = hip.lib(), hip.C.c_void_p()
+    hip.check(L.cldnn_hip_engine_record_begin(eng.h))
+    call(op, x, got)
+    hip.check(L.cldnn_hip_engine_record_end(eng.h, hip.C.byref(rec)))
+    scratch = op.info().workspace_bytes
+    used = L.cldnn_hip_engine_used_memory(eng.h)
+    op.close()
+    assert L.cldnn_hip_engine_used_memory(eng.h) == used
+    # memory of the size that would have been given back, taken by others
+    others = [ops.Buffer(eng, scratch) for _ in range(4)]
+    for _ in range(3):
+        got.zero_()
+        torch.cuda.synchronize()
+        hip.check(L.cldnn_hip_recording_enqueue(rec))
+        eng.finish()
+        assert torch.equal(got, want)
+    for b in others:
+        assert (b.read((scratch // 4,), "i32") == 0).all()
+        b.close()
+    used = L.cldnn_hip_engine_used_memory(eng.h)
+    hip.check(L.cldnn_hip_recording_release(rec))
+    assert L.cldnn_hip_engine_used_memory(eng.h) == used - scratch
+
+
+def test_operands_in_pinned_memory(eng):
+    a, w = (random(generator(n), n, 64, dtype="f16") for n in (3, 40))
+    out, far = torch.empty(3, 40, dtype=torch.float16).pin_memory(), torch.empty(3, 40, dtype=torch.float16, device="cuda")
+    op = ops.Matmul(eng, ops.matmul_desc(3, 40, 64, "f16"))
+    run(eng, op, a.pin_memory(), w.cuda(), out)
+    run(eng, op, a.cuda(), w.cuda(), far)
+    assert torch.equal(out, far.cpu())
+    with pytest.raises(hip.HipError) as err:
+        op.enqueue(a, w.cuda(), far)
+    assert err.value.status == INVALID_ARG
     op.close()
