@@ -212,7 +212,12 @@ def to_type(values, dtype):
     """numpy array of the bits of `values` in an operator's type; bf16, which numpy has not, as uint16 rounded to nearest even"""
     dt = _type(dtype)
     if dt == BF16:
-        bits = np.ascontiguousarray(values, np.float32).view(np.uint32)
+        with np.errstate(over="ignore"):
+            single = np.ascontiguousarray(values, np.float32)
+        bits = single.view(np.uint32)
+        if np.asarray(values).dtype == np.float64:  # rounded to odd first, so that what follows is the one rounding
+            rest = single != values
+            bits = np.where(rest & np.isfinite(single), (bits - (np.abs(single) > np.abs(values))) | 1, bits).astype(np.uint32)
         rounded = ((bits + 0x7fff + ((bits >> 16) & 1)) >> 16).astype(np.uint16)
         return np.where(np.isnan(values), np.uint16(0x7fc0), rounded)
     return np.ascontiguousarray(values, {F32: np.float32, F16: np.float16, I32: np.int32}[dt])

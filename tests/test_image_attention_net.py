@@ -56,6 +56,19 @@ def test_bf16_bits_round_to_nearest_even():
     assert ops.to_type(np.array([np.nan], np.float32), "bf16")[0] == 0x7fc0
 
 
+def test_bf16_bits_of_64_bit_values_are_rounded_once():
+    # next to the middle of two bf16 values, nearer than 32 bits can tell
+    r = np.random.default_rng(3)
+    middles = ((r.integers(0x0080, 0x7f00, 500).astype(np.uint32) << 16) | 0x8000).view(np.float32).astype(np.float64)
+    for sign in (1, -1):
+        for off, up in ((1 + 2.0 ** -40, True), (1 - 2.0 ** -40, False)):
+            values = sign * middles * off
+            bits = ops.to_type(values, "bf16").astype(np.uint32) << 16
+            assert np.array_equal(np.abs(bits.view(np.float32)) > middles, np.full(500, up))
+    assert np.array_equal(ops.to_type(middles, "bf16") & 1, np.zeros(500))  # the middle itself: to even
+    assert np.array_equal(ops.to_type(np.array([1e300, -1e300, np.inf, np.nan, 0.0, -0.0, 1e-300]), "bf16"), np.array([0x7f80, 0xff80, 0x7f80, 0x7fc0, 0, 0x8000, 0], np.uint16))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,half_ulp", [("f16", 2.0 ** -11), ("bf16", 2.0 ** -8)])
 @pytest.mark.parametrize("batch,height,width,blocks", [(1, 56, 56, 1), (3, 72, 40, 2)])
