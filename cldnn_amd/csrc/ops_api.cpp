@@ -75,8 +75,8 @@ void enqueue(cldnn_hip_operator op, F&& launch)
     if (op->info.launches > 1) alone.lock();
     // a recording's kernels go on using the object's memory: it holds the object
     if (op->workspace && op->engine->launch_stream() != op->engine->stream) {
-        (void)cldnn_hip_operator_retain(op);
         op->engine->hold([op] { (void)cldnn_hip_operator_release(op); });
+        op->refs.fetch_add(1);
     }
     launch(op->engine->launch_stream());
 }
