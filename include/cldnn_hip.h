@@ -72,7 +72,7 @@ cldnn_hip_status cldnn_hip_engine_finish(cldnn_hip_engine e);
 /* A recording: between record_begin and record_end the launches that the CALLING THREAD makes on this engine are collected
  * instead of enqueued (a HIP graph); nothing but launches may be made meanwhile.  recording_enqueue puts all of them on the
  * engine's stream with one call, as often as wanted; the pointers they were made with must stay valid until the recording
- * is released.  A stream that is being captured by the application takes no recording (CLDNN_HIP_ERROR, nothing enqueued):
+ * is released (the operators of cldnn_hip_ops.h whose memory it uses it holds itself).  A stream that is being captured by the application takes no recording (CLDNN_HIP_ERROR, nothing enqueued):
  * the launches are made one by one there. */
 typedef struct cldnn_hip_recording_s* cldnn_hip_recording;
 cldnn_hip_status cldnn_hip_engine_record_begin(cldnn_hip_engine e);
