@@ -1,0 +1,220 @@
+// Norms before and after a block, with its gate and residual scale:
+//   z = post(branch) * post_weight + post_bias,  y = residual_scale * x + gate * z,  h = (norm(y) * weight + bias) * (1 + scale) + shift
+//
+// One pass: a token's row is read once and held in registers; the mean is taken first, then the squares around it, so that a mean far
+// from zero costs no digits.
+#include "row_kernel.h"
+
+namespace chip {
+
+struct BlockNormArgs {
+    int64_t tokens;
+    int32_t C, per_image;  // per_image 0: one image
+    int32_t x_type, branch_type, out_type, mod_type;
+    int32_t norm, post;
+    float epsilon, post_epsilon, residual_scale;
+    int64_t x_pitch, branch_pitch, y_pitch, out_pitch, gate_pitch, scale_pitch, shift_pitch;
+};
+
+namespace {
+struct BlockNormPlan : OperatorPlan {
+    BlockNormArgs a{};
+    RowShape shape{};
+};
+}  // namespace
+
+__device__ inline int block_norm_size(int type) { return type == CLDNN_HIP_S8 ? 1 : type == CLDNN_HIP_F32 ? 4 : 2; }
+
+// Values of a row, zeros from C on, become their unit form; two slots of LDS.
+template <int LANES, int NV>
+__device__ __forceinline__ void block_norm_unit(float (&v)[NV][8], int kind, int C, float epsilon, int lane, float (*slot)[LANES < 64 ? 1 : LANES / 64])
+{
+    if (kind == CLDNN_HIP_TOKEN_NORM_NONE) return;
+    if (kind == CLDNN_HIP_TOKEN_NORM_LAYER) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += v[i][j];
+        const float mean = row_sum<LANES>(sum, slot[0]) / (float)C;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = (lane + i * LANES) * 8 + j < C ? v[i][j] - mean : 0.0f;
+    }
+    float squares = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) squares = __builtin_fmaf(v[i][j], v[i][j], squares);
+    const float factor = 1.0f / __builtin_sqrtf(row_sum<LANES>(squares, slot[1]) / (float)C + epsilon);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] *= factor;
+}
+
+template <int LANES, int NV>
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void block_norm_kernel(BlockNormArgs a, BlockNormPointers p)
+{
+    constexpr int THREADS = LANES < 256 ? 256 : LANES;
+    __shared__ float slot[5][LANES < 64 ? 1 : LANES / 64];
+    const int lane = threadIdx.x & (LANES - 1);
+    const int64_t row = (int64_t)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
+    if (row >= a.tokens) return;  // whole groups: nobody waits for them
+    const int64_t image = a.per_image ? (uint32_t)row / (uint32_t)a.per_image : 0;
+    const auto at = [](const void* base, int64_t elements, int type) { return (const char*)base + elements * block_norm_size(type); };
+    const char* x_row = at(p.x, row * a.x_pitch, a.x_type);
+    const bool has_branch = a.branch_type != CLDNN_HIP_NO_TYPE;
+    RowRaw x[NV], branch[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i] = row_load(x_row, a.x_type, (lane + i * LANES) * 8, a.C);
+    float v[NV][8];
+    if (has_branch) {
+        const char* branch_row = at(p.branch, row * a.branch_pitch, a.branch_type);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) branch[i] = row_load(branch_row, a.branch_type, (lane + i * LANES) * 8, a.C);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) row_values(branch[i], a.branch_type, v[i]);
+        block_norm_unit<LANES, NV>(v, a.post, a.C, a.post_epsilon, lane, slot);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + i * LANES) * 8;
+            float f[8];
+            if (p.post_weight) {
+                row_floats(p.post_weight, c, a.C, f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] *= f[j];
+            }
+            if (p.post_bias) {
+                row_floats(p.post_bias, c, a.C, f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] += f[j];
+            }
+            if (p.gate) {
+                row_values(row_load(at(p.gate, image * a.gate_pitch, a.mod_type), a.mod_type, c, a.C), a.mod_type, f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] *= f[j];
+            }
+            row_values(x[i], a.x_type, f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = __builtin_fmaf(a.residual_scale, f[j], v[i][j]);
+            if (p.y && c < a.C) row_store((char*)p.y + row * a.y_pitch * block_norm_size(a.x_type), a.x_type, c, a.C, v[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) row_values(x[i], a.x_type, v[i]);
+    }
+    if (a.out_type == CLDNN_HIP_NO_TYPE) return;
+    block_norm_unit<LANES, NV>(v, a.norm, a.C, a.epsilon, lane, slot + 2);
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (lane + i * LANES) * 8;
+        float f[8];
+        if (p.weight) {
+            row_floats(p.weight, c, a.C, f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] *= f[j];
+        }
+        if (p.bias) {
+            row_floats(p.bias, c, a.C, f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] += f[j];
+        }
+        if (p.scale) {
+            row_values(row_load(at(p.scale, image * a.scale_pitch, a.mod_type), a.mod_type, c, a.C), a.mod_type, f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] *= 1.0f + f[j];
+        }
+        if (p.shift) {
+            row_values(row_load(at(p.shift, image * a.shift_pitch, a.mod_type), a.mod_type, c, a.C), a.mod_type, f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] += f[j];
+        }
+        most = row_magnitude(v[i], most);
+    }
+    if (a.out_type == CLDNN_HIP_S8) {
+        const RowSteps steps = row_steps(row_most<LANES>(most, slot[4]));
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + i * LANES) * 8;
+            if (c < a.C) row_store_s8((int8_t*)p.out + row * a.out_pitch + c, a.C - c, v[i], steps);
+        }
+        if (lane == 0) p.out_scales[row] = steps.scale;
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + i * LANES) * 8;
+            if (c < a.C) row_store((char*)p.out + row * a.out_pitch * block_norm_size(a.out_type), a.out_type, c, a.C, v[i]);
+        }
+    }
+}
+
+std::unique_ptr<OperatorPlan> block_norm_plan(const cldnn_hip_engine_s&, const cldnn_hip_block_norm_desc& d, cldnn_hip_operator_info& info)
+{
+    CHIP_REQUIRE(d.tokens > 0 && d.features > 0 && d.tokens_per_image >= 0, CLDNN_HIP_INVALID_ARG, "block norm: sizes must be positive");
+    CHIP_REQUIRE(d.features <= ROW_MOST, CLDNN_HIP_UNSUPPORTED_SIZE, "block norm: too many features, more than 32768");
+    const bool branch = d.branch_dtype != CLDNN_HIP_NO_TYPE, out = d.out_dtype != CLDNN_HIP_NO_TYPE, quantized = d.out_dtype == CLDNN_HIP_S8;
+    const int64_t x_size = float_size(d.dtype, "block norm"), branch_size = branch ? float_size(d.branch_dtype, "block norm") : 0;
+    const int64_t out_size = !out ? 0 : quantized ? 1 : float_size(d.out_dtype, "block norm");
+    if (d.modulation_dtype != CLDNN_HIP_NO_TYPE) (void)float_size(d.modulation_dtype, "block norm");
+    const auto known = [](int norm) { return norm >= CLDNN_HIP_TOKEN_NORM_NONE && norm <= CLDNN_HIP_TOKEN_NORM_RMS; };
+    CHIP_REQUIRE(known(d.norm) && known(d.post), CLDNN_HIP_INVALID_ARG, "block norm: unknown norm");
+    CHIP_REQUIRE(d.epsilon >= 0.0f && d.post_epsilon >= 0.0f, CLDNN_HIP_INVALID_ARG, "block norm: epsilon must not be negative");
+    CHIP_REQUIRE(branch || out, CLDNN_HIP_INVALID_ARG, "block norm: neither a branch nor an output");
+    CHIP_REQUIRE(branch || (d.post == CLDNN_HIP_TOKEN_NORM_NONE && d.residual_scale == 1.0f), CLDNN_HIP_INVALID_ARG, "block norm: a norm or scale of a branch without one");
+    CHIP_REQUIRE(out || d.norm == CLDNN_HIP_TOKEN_NORM_NONE, CLDNN_HIP_INVALID_ARG, "block norm: a norm without an output");
+    std::unique_ptr<BlockNormPlan> plan(new BlockNormPlan());
+    BlockNormArgs& a = plan->a;
+    a.tokens = d.tokens, a.C = d.features, a.per_image = d.tokens_per_image;
+    a.x_type = d.dtype, a.branch_type = d.branch_dtype, a.out_type = d.out_dtype, a.mod_type = d.modulation_dtype;
+    a.norm = d.norm, a.post = d.post, a.epsilon = d.epsilon, a.post_epsilon = d.post_epsilon, a.residual_scale = d.residual_scale;
+    const auto pitch = [&](int64_t stride) {
+        CHIP_REQUIRE(stride == 0 || stride >= d.features, CLDNN_HIP_INVALID_ARG, "block norm: a stride shorter than its row");
+        return stride ? stride : d.features;
+    };
+    a.x_pitch = pitch(d.x_stride), a.branch_pitch = pitch(d.branch_stride), a.y_pitch = pitch(d.y_stride), a.out_pitch = pitch(d.out_stride);
+    a.gate_pitch = pitch(d.gate_stride), a.scale_pitch = pitch(d.scale_stride), a.shift_pitch = pitch(d.shift_stride);
+    plan->shape = row_shape(d.features);
+    const int64_t blocks = plan->shape.blocks(d.tokens);
+    check_grid(blocks, plan->shape.threads(), "block norm");
+    info.launches = 1, info.grid = (int32_t)blocks, info.block = plan->shape.threads(), info.lds_bytes = plan->shape.lanes > 64 ? 5 * plan->shape.lanes / 64 * 4 : 0;
+    const int64_t values = d.tokens * d.features;
+    info.ops = 20 * values;
+    info.bytes = values * (x_size + (branch ? branch_size + x_size : 0) + out_size) + (quantized ? 4 * d.tokens : 0);
+    snprintf(info.kernel_name, sizeof info.kernel_name, "block_norm<%dx%d>", plan->shape.lanes, plan->shape.vectors);
+    return plan;
+}
+
+void block_norm_launch(hipStream_t s, const OperatorPlan& plan, const BlockNormPointers& of)
+{
+    const BlockNormPlan& p = static_cast<const BlockNormPlan&>(plan);
+    const BlockNormArgs& a = p.a;
+    BlockNormPointers given = of;
+    // what the description has not is not looked at
+    if (a.branch_type == CLDNN_HIP_NO_TYPE) given.branch = nullptr, given.post_weight = given.post_bias = nullptr, given.gate = nullptr, given.y = nullptr;
+    if (a.out_type == CLDNN_HIP_NO_TYPE) given.out = nullptr, given.weight = given.bias = nullptr, given.scale = given.shift = nullptr;
+    if (a.out_type != CLDNN_HIP_S8) given.out_scales = nullptr;
+    if (a.mod_type == CLDNN_HIP_NO_TYPE) given.gate = given.scale = given.shift = nullptr;
+    CHIP_REQUIRE((a.branch_type == CLDNN_HIP_NO_TYPE || given.branch) && (a.out_type == CLDNN_HIP_NO_TYPE ? given.y != nullptr : given.out != nullptr) &&
+                     (a.out_type != CLDNN_HIP_S8 || given.out_scales),
+                 CLDNN_HIP_INVALID_ARG, "null device pointer");
+    CHIP_REQUIRE(given.y != given.x || a.y_pitch == a.x_pitch, CLDNN_HIP_INVALID_ARG, "block norm: y in the place of x with another stride");
+    const int x_align = float_size(a.x_type, "");
+    check_aligned(given.x, x_align, "x"), check_aligned(given.y, x_align, "y");
+    if (given.branch) check_aligned(given.branch, float_size(a.branch_type, ""), "branch");
+    if (given.out && a.out_type != CLDNN_HIP_S8) check_aligned(given.out, float_size(a.out_type, ""), "output");
+    if (a.mod_type != CLDNN_HIP_NO_TYPE) {
+        const int to = float_size(a.mod_type, "");
+        check_aligned(given.gate, to, "gate"), check_aligned(given.scale, to, "scale"), check_aligned(given.shift, to, "shift");
+    }
+    check_aligned(given.post_weight, 4, "post_weight"), check_aligned(given.post_bias, 4, "post_bias"), check_aligned(given.weight, 4, "weight"), check_aligned(given.bias, 4, "bias");
+    check_aligned(given.out_scales, 4, "out_scales");
+    with_row_shape(p.shape, [&](auto lanes, auto vectors) {
+        hipLaunchKernelGGL((block_norm_kernel<decltype(lanes)::value, decltype(vectors)::value>), dim3((unsigned)p.shape.blocks(a.tokens)), dim3(p.shape.threads()), 0, s, a, given);
+    });
+    CHIP_CHECK(hipGetLastError());
+}
+
+}  // namespace chip

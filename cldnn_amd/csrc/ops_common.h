@@ -115,7 +115,12 @@ __device__ inline void act_apply(float (&v)[N], const Act& a)
 }
 
 // ----------------------------------------------------------------------------- operator objects
-enum OperatorKind { OP_GROUP_NORM, OP_MATMUL, OP_ROTARY, OP_ATTENTION };
+enum OperatorKind { OP_GROUP_NORM, OP_MATMUL, OP_ROTARY, OP_ATTENTION, OP_QUANTIZE, OP_MATMUL_S8, OP_BLOCK_NORM };
+
+// What create worked out for an operator of another library than that of the object.
+struct OperatorPlan {
+    virtual ~OperatorPlan() = default;
+};
 
 struct NormPlan;
 struct MatmulPlan;
@@ -135,6 +140,7 @@ struct cldnn_hip_operator_s {
     chip::MatmulPlan* matmul = nullptr;
     chip::RotaryPlan* rotary = nullptr;
     chip::AttentionPlan* attention = nullptr;
+    std::unique_ptr<chip::OperatorPlan> plan;
     ~cldnn_hip_operator_s();
 };
 

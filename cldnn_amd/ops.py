@@ -17,9 +17,9 @@ from . import hip
 LIB_PATH = os.path.join(os.path.dirname(hip.LIB_PATH), "libcldnn_hip_ops.so")
 
 F32, F16, BF16, I32, NO_TYPE = hip.F32, 4, 5, hip.I32, hip.NO_TYPE
-DT_NAME = {"f32": F32, "f16": F16, "bf16": BF16, "i32": I32}
-TORCH_NAME = {F32: "torch.float32", F16: "torch.float16", BF16: "torch.bfloat16", I32: "torch.int32"}
-SIZE = {F32: 4, F16: 2, BF16: 2, I32: 4}
+DT_NAME = {"f32": F32, "f16": F16, "bf16": BF16, "i32": I32, "s8": hip.S8}
+TORCH_NAME = {F32: "torch.float32", F16: "torch.float16", BF16: "torch.bfloat16", I32: "torch.int32", hip.S8: "torch.int8"}
+SIZE = {F32: 4, F16: 2, BF16: 2, I32: 4, hip.S8: 1}
 POSITION_NAME = {"i32": I32, "f32": F32}
 ACT_NAME = dict(hip.ACT_NAME, silu=4, gelu=5, gelu_tanh=6)
 PAIRING_NAME = {"interleaved": 0, "halves": 1, "halves_per_axis": 2}
@@ -187,14 +187,14 @@ class Buffer:
         return self
 
     def read(self, shape, dtype):
-        """the first values as numpy float32 (i32: int32); waits for the engine"""
-        n = {F32: np.float32, I32: np.int32, F16: np.float16, BF16: np.uint16}[_type(dtype)]
+        """the first values as numpy float32 (i32: int32, s8: int8); waits for the engine"""
+        n = {F32: np.float32, I32: np.int32, F16: np.float16, BF16: np.uint16, hip.S8: np.int8}[_type(dtype)]
         a = np.empty(shape, n)
         assert a.nbytes <= self.nbytes, (a.nbytes, self.nbytes)
         hip.check(hip.lib().cldnn_hip_buffer_read(self.h, 0, a.ctypes.data, a.nbytes))
         if _type(dtype) == BF16:
             return (a.astype(np.uint32) << 16).view(np.float32)
-        return a if _type(dtype) == I32 else a.astype(np.float32)
+        return a if _type(dtype) in (I32, hip.S8) else a.astype(np.float32)
 
     def close(self):
         if self.h:
@@ -220,18 +220,20 @@ def to_type(values, dtype):
             bits = np.where(rest & np.isfinite(single), (bits - (np.abs(single) > np.abs(values))) | 1, bits).astype(np.uint32)
         rounded = ((bits + 0x7fff + ((bits >> 16) & 1)) >> 16).astype(np.uint16)
         return np.where(np.isnan(values), np.uint16(0x7fc0), rounded)
-    return np.ascontiguousarray(values, {F32: np.float32, F16: np.float16, I32: np.int32}[dt])
+    return np.ascontiguousarray(values, {F32: np.float32, F16: np.float16, I32: np.int32, hip.S8: np.int8}[dt])
 
 
 class Operator:
     """What the operators have in common: the object behind the handle."""
 
+    _library = staticmethod(lib)  # whose entry points the kind has
+
     def __init__(self, engine, kind, desc):
         self.engine, self.desc, self.h = engine, desc, None
         h = _P()
-        hip.check(getattr(lib(), "cldnn_hip_%s_create" % kind)(engine.h, C.byref(desc), C.byref(h)))
+        hip.check(getattr(self._library(), "cldnn_hip_%s_create" % kind)(engine.h, C.byref(desc), C.byref(h)))
         self.h = h
-        self._enqueue = getattr(lib(), "cldnn_hip_%s_enqueue" % kind)
+        self._enqueue = getattr(self._library(), "cldnn_hip_%s_enqueue" % kind)
         self._address = [_address_of(o, engine.device) for o in self._operands(desc)]  # in the entry point's order
 
     def info(self):
