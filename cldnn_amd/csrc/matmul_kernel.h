@@ -25,6 +25,7 @@ struct MatmulS8Args : MatmulArgs {
     const float *a_scales, *w_scales;  // nullptr: 1
     int32_t a_each, w_each;            // 1: one to a row; 0: one for all
     int32_t out_type, res_type;        // CLDNN_HIP_F32, F16, BF16
+    int32_t out_runs;                  // result and residual are whole runs of matmul_run(out_type) values at any place of a tile
 };
 
 // What the kernels ask of an operand's type: a 16-byte piece as the matrix instruction takes it, its sums, the arguments of its product.
@@ -37,6 +38,7 @@ template <typename T> struct MatmulType {
     typedef float One;
     typedef MatmulArgs Args;
     static constexpr int E = 8;  // values of a piece
+    static constexpr bool SHORT = false;  // form of the activations
 };
 template <> struct MatmulType<int8_t> {
     typedef v4i V;
@@ -45,6 +47,7 @@ template <> struct MatmulType<int8_t> {
     typedef int32_t One;
     typedef MatmulS8Args Args;
     static constexpr int E = 16;
+    static constexpr bool SHORT = true;
 };
 __device__ inline v4i mfma16(v4i a, v4i b, v4i c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
@@ -142,7 +145,7 @@ __device__ __forceinline__ void matmul_write_row(const MatmulS8Args& a, float (&
         else matmul_read((const __bf16*)a.residual + at, valid, r);
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] += r[i];
-        act_apply(v, a.act2);
+        act_apply<MatmulType<T>::SHORT>(v, a.act2);
     }
     const int64_t at = m * a.o_pitch + n0;
     if (a.out_type == CLDNN_HIP_F32) matmul_write((float*)out + at, valid, v);
@@ -289,7 +292,7 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_split_kernel(typename Matmu
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] += b[i];
         }
-        act_apply(v, a.act);
+        act_apply<MatmulType<T>::SHORT>(v, a.act);
         matmul_write_row<T>(a, v, m0 + row, n, out);
     }
 }
@@ -322,9 +325,170 @@ __global__ __launch_bounds__(256) void matmul_join_kernel(typename MatmulType<T>
 #pragma unroll
         for (int l = 0; l < 4; ++l) v[l] += b[l];
     }
-    act_apply(v, a.act);
+    act_apply<MatmulType<T>::SHORT>(v, a.act);
     matmul_write_row<T>(a, v, m, n, out);
 }
+
+// ----------------------------------------------------------------------------- the end of a tile of int8 operands
+// Values of a run: 16 bytes of the result, which a lane stores as one piece beside those of its neighbours.  Four lanes write 64 bytes
+// without a gap then; 16 neighbours to a lane, as the float products have them, are written in pieces 32 bytes apart, and 25088 x 1024 ->
+// 4096 took twice the requests to memory.
+__device__ inline int matmul_run(int type) { return type == CLDNN_HIP_F32 ? 4 : 8; }
+
+// Where the g-th four of a lane's 16 values lie among the wave's 64 features.
+__device__ inline int matmul_four(const MatmulS8Args& a, int g, int q) { return a.out_type == CLDNN_HIP_F32 ? 16 * g + 4 * q : 32 * (g >> 1) + 8 * q + 4 * (g & 1); }
+__device__ inline int matmul_feature(const MatmulS8Args& a, int b) { return matmul_four(a, b >> 4, b >> 2 & 3) + (b & 3); }
+
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+// f(T()) for one of the float types
+template <typename F>
+__device__ __forceinline__ void matmul_typed(int type, F&& f)
+{
+    if (type == CLDNN_HIP_F32) f(float());
+    else if (type == CLDNN_HIP_F16) f(_Float16());
+    else f(__bf16());
+}
+
+// A lane's 16 values of a row of the residual as they lie in memory; 16-bit types fill half.
+typedef uint32_t v16u __attribute__((ext_vector_type(16)));
+template <typename T>
+__device__ __forceinline__ void matmul_add_row(const v16u& row, float (&v)[16])
+{
+    typedef T vec __attribute__((ext_vector_type(64 / sizeof(T))));
+    const vec x = __builtin_bit_cast(vec, row);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] += (float)x[i];
+}
+
+// The sums of a wave, 16 MB rows from m on x 64 features from n on: scales, bias, activation, residual, its activation, the result.  The
+// residual's row is asked for one row ahead.  spare: LDS of the wave, 16 x 64 floats, that nobody reads any more; the result goes
+// through it where it is no whole runs, one element to a lane.
+template <int MB>
+__device__ __forceinline__ void matmul_finish_s8(const MatmulS8Args& a, const v4i (&sum)[4][MB], int m, int n, int lane, float* spare, void* out)
+{
+    const int q = lane >> 4, r = lane & 15;
+    const bool fours = a.out_type == CLDNN_HIP_F32;
+    const int res_size = a.res_type == CLDNN_HIP_F32 ? 4 : 2, out_size = fours ? 4 : 2;
+    const auto buffer = [&](const void* base, int64_t pitch, int size) {
+        return __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<void*>(base) + (m * pitch + n) * size, 0, 0x7fffffff, 0x00020000);
+    };
+    const auto from = buffer(a.residual, a.r_pitch, res_size), to = buffer(out, a.o_pitch, out_size);
+    // the place of four features of a row; behind the buffer's end for what is not in the result
+    const auto place = [&](int i, int g, int64_t pitch, int size) {
+        const int feature = matmul_four(a, g, q);
+        return m + 16 * i + r < a.m && n + feature < a.n ? (16 * i + r) * (int)(pitch * size) + feature * size : (int)0x80000000;
+    };
+    const bool runs = a.out_runs, residual = a.residual && runs;
+    const auto fetch = [&](int i) {
+        v16u row{};
+        if (res_size == 4) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const v4u y = __builtin_amdgcn_raw_buffer_load_b128(from, place(i, g, a.r_pitch, 4), 0, 0);
+                row[4 * g] = y[0], row[4 * g + 1] = y[1], row[4 * g + 2] = y[2], row[4 * g + 3] = y[3];
+            }
+        } else if (fours) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const v2u y = __builtin_amdgcn_raw_buffer_load_b64(from, place(i, g, a.r_pitch, 2), 0, 0);
+                row[2 * g] = y[0], row[2 * g + 1] = y[1];
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const v4u y = __builtin_amdgcn_raw_buffer_load_b128(from, place(i, 2 * g, a.r_pitch, 2), 0, 0);
+                row[4 * g] = y[0], row[4 * g + 1] = y[1], row[4 * g + 2] = y[2], row[4 * g + 3] = y[3];
+            }
+        }
+        return row;
+    };
+    v16u now{}, then{};
+    if (residual) now = fetch(0);
+    float scale[16], bias[16], row_scale[MB];
+    const float all = a.w_scales && !a.w_each ? *a.w_scales : 1.0f;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) row_scale[i] = matmul_row_scale(a, m + 16 * i + r);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int f = n + matmul_four(a, g, q);
+        float s[4] = {all, all, all, all}, b[4] = {};
+        if (a.w_each && f < a.n) matmul_read(a.w_scales + f, a.n - f, s);
+        if (a.bias && f < a.n) matmul_read(a.bias + f, a.n - f, b);
+#pragma unroll
+        for (int l = 0; l < 4; ++l) scale[4 * g + l] = s[l], bias[4 * g + l] = b[l];
+    }
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        if (residual && i + 1 < MB) then = fetch(i + 1);
+        float v[16];
+#pragma unroll
+        for (int l = 0; l < 16; ++l) v[l] = (float)sum[l / 4][i][l % 4] * row_scale[i] * scale[l] + bias[l];
+        act_apply<true>(v, a.act);
+        if (residual) {
+            matmul_typed(a.res_type, [&](auto t) { matmul_add_row<decltype(t)>(now, v); });
+            if (a.act2.kind != CLDNN_HIP_ACT_NONE) act_apply<true>(v, a.act2);
+            now = then;
+        }
+        if (runs) {
+            matmul_typed(a.out_type, [&](auto t) {
+                typedef decltype(t) T;
+                constexpr int R = 16 / sizeof(T);
+                typedef T vec __attribute__((ext_vector_type(R)));
+#pragma unroll
+                for (int l = 0; l < 16; l += R) {
+                    vec x;
+#pragma unroll
+                    for (int k = 0; k < R; ++k) x[k] = (T)v[l + k];
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, x), to, place(i, l / 4, a.o_pitch, sizeof(T)), 0, 0);
+                }
+            });
+            continue;
+        }
+#pragma unroll
+        for (int l = 0; l < 16; ++l) spare[r * 64 + matmul_four(a, l / 4, q) + l % 4] = v[l];
+        __builtin_amdgcn_wave_barrier();
+        for (int k = 0; k < 16; ++k) {
+            const int row = m + 16 * i + k;
+            if (row >= a.m || n + lane >= a.n) break;
+            float x[1] = {spare[k * 64 + lane]};
+            if (a.residual) {
+                const int64_t at = row * a.r_pitch + n + lane;
+                matmul_typed(a.res_type, [&](auto t) { x[0] += (float)((const decltype(t)*)a.residual)[at]; });
+                if (a.act2.kind != CLDNN_HIP_ACT_NONE) act_apply<true>(x, a.act2);
+            }
+            const int64_t at = row * a.o_pitch + n + lane;
+            matmul_typed(a.out_type, [&](auto t) { ((decltype(t)*)out)[at] = (decltype(t))x[0]; });
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// The sums of a wave, 16 MB rows from m on x 64 features from n on, of float operands: bias, activation, residual, the result.
+template <typename T, int MB>
+__device__ __forceinline__ void matmul_finish_rows(const MatmulArgs& a, const v4f (&sum)[4][MB], int m, int n, int lane, void* out)
+{
+    const int q = lane >> 4, r = lane & 15;
+    n += 16 * q;
+    float bias[16] = {};
+    if (a.bias && n < a.n) matmul_read(a.bias + n, a.n - n, bias);
+    act_choose(a.act.kind, [&](auto kind) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            float v[16];
+#pragma unroll
+            for (int l = 0; l < 16; ++l) v[l] = sum[l / 4][i][l % 4] + bias[l];
+#pragma unroll
+            for (int l = 0; l < 16; ++l) v[l] = act_one<decltype(kind)::value>(v[l], a.act.m, a.act.n);
+            matmul_write_row<T>(a, v, m + i * 16 + r, n, out);
+        }
+    });
+}
+
+// Which of a wave's 64 features the b-th of its rows of weights is: 16 (r / 4) + 4 t + r % 4 for row 16 t + r.  The four results that the
+// matrix instruction leaves in a lane are neighbours, and so are those of the four blocks t: 16 features of one row of the result.
+__device__ inline int matmul_feature(const MatmulArgs&, int b) { return 16 * (b >> 2 & 3) + 4 * (b >> 4) + (b & 3); }
 
 // BM x BN of the result to a workgroup of WM x WN waves, 16 MB rows x 64 features to a wave.  Both operands come 64 deep into two LDS
 // buffers by direct loads, one step ahead of the one that is multiplied.  A row of 64 values is eight pieces of 16 bytes; piece c
@@ -334,8 +498,6 @@ __global__ __launch_bounds__(256) void matmul_join_kernel(typename MatmulType<T>
 // units are busy in 72 % of the time, at the 1.5 GHz that the power limit leaves.  On the way there: 32x32x16 instructions 882 us,
 // both halves of the waves in step 926, tiles of a die in a row instead of a block 959.  25088 x 1024 -> 4096 with a gelu 232 us, its
 // product alone 203: seven rounds of 16 steps, 4 us of each the prologue and the stores, 4 the gelu, which nothing overlaps.
-// Row 16 t + r of a wave's 64 rows of weights is feature 16 (r / 4) + 4 t + r % 4 of its 64: the four results that the matrix
-// instruction leaves in a lane are neighbours, and so are those of the four blocks t: 16 features of one row of the result.
 template <typename T, int WM, int WN, int MB, int ST, int KG>
 __global__ __launch_bounds__(64 * WM * WN * KG, 2) void matmul_tile_kernel(typename MatmulType<T>::Args a, const T* x, const T* w, void* out)
 {
@@ -366,7 +528,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void matmul_tile_kernel(typen
 #pragma unroll
     for (int i = 0; i < WL; ++i) {
         const int row = (i * WAVES + wave) * 8 + (lane >> 3), b = row & 63;
-        const int feature = (row & ~63) + 16 * (b >> 2 & 3) + 4 * (b >> 4) + (b & 3);
+        const int feature = (row & ~63) + matmul_feature(a, b);
         wo[i] = min(feature, a.n - 1 - n0) * (int)(a.w_pitch * S) + 16 * ((lane & 7) ^ (row >> 1 & 7));
     }
     // every load of a wave starts at the same multiple of 8 modulo 16
@@ -442,7 +604,6 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void matmul_tile_kernel(typen
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    const int n = n0 + wn * 64 + 16 * q;
     if constexpr (KG > 1) {
         // the groups' sums meet in LDS, in the order of the groups: group g finishes every KG-th block of rows
         static_assert(KG * WAVES * MB * 256 <= KG * ST * (BM + BN) * 8 && (KG - 1) * MB >= 1, "the sums fit where the operands were");
@@ -454,42 +615,24 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void matmul_tile_kernel(typen
             for (int j = 0; j < 4; ++j) sums[(((group * WAVES + wave) * MB + i) * 4 + j) * 64 + lane] = acc[j][i];
         __syncthreads();
         for (int i = group; i < MB; i += KG) {
-            typename Type::One sum[16];
+            Sum sum[4][1];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                Sum t = sums[((wave * MB + i) * 4 + j) * 64 + lane];
+                sum[j][0] = sums[((wave * MB + i) * 4 + j) * 64 + lane];
 #pragma unroll
-                for (int g = 1; g < KG; ++g) t += sums[(((g * WAVES + wave) * MB + i) * 4 + j) * 64 + lane];
-#pragma unroll
-                for (int l = 0; l < 4; ++l) sum[4 * j + l] = t[l];
+                for (int g = 1; g < KG; ++g) sum[j][0] += sums[(((g * WAVES + wave) * MB + i) * 4 + j) * 64 + lane];
             }
-            const int m = m0 + (wm * MB + i) * 16 + r;
-            float v[16], bias[16] = {};
-            const MatmulColumns<T, 16> columns(a, n);
-            const float scale = matmul_row_scale(a, m);
-            if (a.bias && n < a.n) matmul_read(a.bias + n, a.n - n, bias);
-#pragma unroll
-            for (int l = 0; l < 16; ++l) v[l] = columns.value(l, sum[l], scale) + bias[l];
-            act_apply(v, a.act);
-            matmul_write_row<T>(a, v, m, n, out);
+            // (this wave has read what lies where its spare memory is, and nobody else reads it)
+            const int m = m0 + (wm * MB + i) * 16, n = n0 + wn * 64;
+            if constexpr (E == 16) matmul_finish_s8(a, sum, m, n, lane, (float*)(sums + (wave * MB + i) * 256), out);
+            else matmul_finish_rows<T>(a, sum, m, n, lane, out);
         }
     } else {
-        const MatmulColumns<T, 16> columns(a, n);
-        float bias[16] = {};
-        if (a.bias && n < a.n) matmul_read(a.bias + n, a.n - n, bias);
-        act_choose(a.act.kind, [&](auto kind) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < MB; ++i) {
-                const int m = m0 + (wm * MB + i) * 16 + r;
-                const float scale = matmul_row_scale(a, m);
-                float v[16];
-#pragma unroll
-                for (int l = 0; l < 16; ++l) v[l] = columns.value(l, acc[l / 4][i][l % 4], scale) + bias[l];
-#pragma unroll
-                for (int l = 0; l < 16; ++l) v[l] = act_one<decltype(kind)::value>(v[l], a.act.m, a.act.n);
-                matmul_write_row<T>(a, v, m, n, out);
-            }
-        });
+        const int m = m0 + wm * MB * 16, n = n0 + wn * 64;
+        if constexpr (E == 16) {
+            if (!a.out_runs) asm volatile("s_barrier" ::: "memory");  // the others' last reads of the operands are done
+            matmul_finish_s8(a, acc, m, n, lane, (float*)lds + wave * 1024, out);
+        } else matmul_finish_rows<T>(a, acc, m, n, lane, out);
     }
 }
 

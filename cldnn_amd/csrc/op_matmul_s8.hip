@@ -6,7 +6,207 @@
 namespace chip {
 
 constexpr int MATMUL_S8_MOST_K = 131071;  // 128 * 128 of each fit 31 bits
+constexpr int64_t MATMUL_S8_RUN_PITCH = 1 << 20;  // 256 rows of it in f32 are within a buffer's reach
 constexpr int64_t MATMUL_S8_PACK = 200ll << 20;  // products from which unaligned operands are copied
+
+// Large products: 32 MB rows x 256 features at a time to a workgroup of 2 x 4 waves, which goes through tiles i, i + grid, .. of the result.
+// The main loop is that of matmul_tile_kernel<2, 4, MB>, whose comment says how the halves of the waves take turns; what is different
+// is the end of a tile.  The next tile's first operands are asked for in front of it, and its stores drain under the next one's products,
+// where a workgroup to a tile waits for all of them before its LDS is free for the next.  Scales and bias are asked for a tile ahead,
+// a value to a thread, and handed out through LDS; every place of the result is an offset that is worked out once.
+// O: the result's type; RES: a residual is added.  The result (and the residual) is whole runs (MatmulS8Args::out_runs).
+template <typename O, bool RES, int MB>
+__global__ __launch_bounds__(512, 2) void matmul_s8_walk_kernel(MatmulS8Args a, const int8_t* x, const int8_t* w, void* out)
+{
+    constexpr int WN = 4, WAVES = 8, BM = 32 * MB, BN = 256, BK = 128;
+    constexpr int XL = (BM / 8 + WAVES - 1) / WAVES, WL = BN / 8 / WAVES;  // loads of a wave: 8 rows each
+    constexpr int R = 16 / sizeof(O), RUNS = 16 / R;
+    __shared__ v4i lds[2 * (BM + BN) * 8];
+    __shared__ float rows[BM], columns[2 * BN];  // of the tile that ends: scales of rows; scales of features, bias
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const v4i *xt = lds, *wt = lds + 2 * BM * 8;
+    const uint32_t xl = lds_address(xt), wl = lds_address(wt);
+    const int q = lane >> 4, r = lane & 15, wm = wave / WN, wn = wave - wm * WN;
+    const int steps = (a.k + BK - 1) / BK, piece = (lane & 7) ^ (q | (wave & 1) << 2);
+    const bool late = wave >= WAVES / 2;
+    // the first of a run of a lane's values among the wave's 64 features
+    const auto run = [&](int k) { return R == 4 ? 16 * k + 4 * q : 32 * k + 8 * q; };
+
+    int m0, n0, xo[XL], wo[WL];
+    v4i xs, ws;
+    float row_value, column_value;
+    const auto aim = [&](int tile) {
+        int tm, tn, t = threadIdx.x;
+        asm volatile("" : "+v"(t));  // (known, all of this would be worked out once for all tiles and kept in scratch memory)
+        matmul_place(a, tile, tm, tn);
+        m0 = tm * BM, n0 = tn * BN;
+        xs = buffer_of(x + (int64_t)m0 * a.a_pitch), ws = buffer_of(w + (int64_t)n0 * a.w_pitch);
+        const int of = (wave << 3) + (t >> 3 & 7);
+#pragma unroll
+        for (int i = 0; i < XL; ++i) xo[i] = min(i * WAVES * 8 + of, a.m - 1 - m0) * (int)a.a_pitch + 16 * piece;
+#pragma unroll
+        for (int i = 0; i < WL; ++i) {
+            const int row = i * WAVES * 8 + of, b = row & 63;
+            const int feature = R == 4 ? b : (b & 32) + 8 * (b >> 2 & 3) + 4 * (b >> 4 & 1) + (b & 3);
+            wo[i] = min((row & ~63) + feature, a.n - 1 - n0) * (int)a.w_pitch + 16 * piece;
+        }
+        row_value = 1.0f, column_value = t < BN ? 1.0f : 0.0f;
+        if (a.a_scales && t < BM) row_value = a.a_scales[a.a_each ? min(m0 + t, a.m - 1) : 0];
+        const int n = min(n0 + (t & (BN - 1)), a.n - 1);
+        if (t < BN) {
+            if (a.w_scales) column_value = a.w_scales[a.w_each ? n : 0];
+        } else if (a.bias) column_value = a.bias[n];
+    };
+    const auto load = [&](int step, int at) {
+        const int behind = step * BK + 16 * piece >= a.k ? (int)0x80000000 : 0;
+#pragma unroll
+        for (int i = 0; i < XL; ++i)
+            if (BM / 8 % WAVES == 0 || i * WAVES + wave < BM / 8) load_lds(xs, xl + at * BM * 128 + (i * WAVES + wave) * 1024, xo[i] | behind, step * BK);
+#pragma unroll
+        for (int i = 0; i < WL; ++i) load_lds(ws, wl + at * BN * 128 + (i * WAVES + wave) * 1024, wo[i] | behind, step * BK);
+    };
+    v4i acc[4][MB], xf[MB], wf[4];
+    const auto read = [&](int round, int at) {
+        const int place = (4 * round + q) ^ (r >> 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) wf[j] = wt[at * BN * 8 + (wn * 64 + j * 16 + r) * 8 + place];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) xf[i] = xt[at * BM * 8 + ((wm * MB + i) * 16 + r) * 8 + place];
+    };
+    const auto multiply = [&]() {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j][i] = mfma16(wf[j], xf[i], acc[j][i]);
+        __builtin_amdgcn_s_setprio(0);
+    };
+    int tile = blockIdx.x;
+    aim(tile);
+    load(0, 0);
+    matmul_arrive<0>();
+    for (;;) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j][i] = v4i{0, 0, 0, 0};
+        if (late) matmul_meet();
+        for (int step = 0, at = 0; step < steps; ++step, at ^= 1) {
+            load(step + 1, at ^ 1);
+            read(0, at);
+            matmul_meet();
+            multiply();
+            matmul_meet();
+            read(1, at);
+            // all reads of this buffer are done and the next step's loads have landed where the late waves end this phase
+            if (late) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            matmul_meet();
+            multiply();
+            if (!late) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            matmul_meet();
+        }
+        if (!late) matmul_meet();
+        // nobody reads or fills the operands' LDS any more
+        if (threadIdx.x < BM) rows[threadIdx.x] = row_value;
+        columns[threadIdx.x] = column_value;
+        const int m = m0 + wm * MB * 16, n = n0 + wn * 64;
+        tile += gridDim.x;
+        const bool more = tile < a.tiles;
+        if (more) {
+            aim(tile);
+            load(0, 0);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+
+        float scale[16], bias[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int f = wn * 64 + (R == 4 ? run(g) : run(g >> 1) + 4 * (g & 1));
+            const v4f s = *(const v4f*)&columns[f], b = *(const v4f*)&columns[BN + f];
+#pragma unroll
+            for (int l = 0; l < 4; ++l) scale[4 * g + l] = s[l], bias[4 * g + l] = b[l];
+        }
+        // Offsets from the wave's first value on.  Rows behind the last are behind the buffer's end, features behind the last are sent there.
+        const auto buffer = [&](const void* base, int64_t pitch, int size) {
+            const int64_t bytes = (a.m - m) * pitch * size;
+            return __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<void*>(base) + (m * pitch + n) * size, 0, m < a.m ? (int)min(bytes, (int64_t)0x7fffffff) : 0, 0x00020000);
+        };
+        const auto place = [&](int k, int64_t pitch, int size) { return n + run(k) < a.n ? r * (int)(pitch * size) + run(k) * size : (int)0x80000000; };
+        const auto to = buffer(out, a.o_pitch, sizeof(O));
+        int at[RUNS];
+#pragma unroll
+        for (int k = 0; k < RUNS; ++k) at[k] = place(k, a.o_pitch, sizeof(O));
+        const int o_step = 16 * (int)(a.o_pitch * sizeof(O));
+        const auto value = [&](int i, float (&v)[16]) {
+            const float row = rows[(wm * MB + i) * 16 + r];
+#pragma unroll
+            for (int l = 0; l < 16; ++l) v[l] = __builtin_fmaf((float)acc[l / 4][i][l % 4] * row, scale[l], bias[l]);
+        };
+        const auto store = [&](int i, const float (&v)[16]) {
+            typedef O vec __attribute__((ext_vector_type(R)));
+#pragma unroll
+            for (int k = 0; k < RUNS; ++k) {
+                vec y;
+#pragma unroll
+                for (int l = 0; l < R; ++l) y[l] = (O)v[k * R + l];
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, y), to, at[k] + i * o_step, 0, 0);
+            }
+        };
+        if constexpr (RES) {
+            const int size = a.res_type == CLDNN_HIP_F32 ? 4 : 2, r_step = 16 * (int)(a.r_pitch * size);
+            const auto from = buffer(a.residual, a.r_pitch, size);
+            int there[RUNS];
+#pragma unroll
+            for (int k = 0; k < RUNS; ++k) there[k] = place(k, a.r_pitch, size);
+            const auto fetch = [&](int i) {
+                v16u y{};
+                const auto four = [&](int g, v4u z) { y[4 * g] = z[0], y[4 * g + 1] = z[1], y[4 * g + 2] = z[2], y[4 * g + 3] = z[3]; };
+                if (size == 4) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        four(g, __builtin_amdgcn_raw_buffer_load_b128(from, there[R == 4 ? g : g >> 1] + i * r_step + (R == 4 ? 0 : 16 * (g & 1)), 0, 0));
+                } else if constexpr (R == 4) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const v2u z = __builtin_amdgcn_raw_buffer_load_b64(from, there[g] + i * r_step, 0, 0);
+                        y[2 * g] = z[0], y[2 * g + 1] = z[1];
+                    }
+                } else {
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) four(g, __builtin_amdgcn_raw_buffer_load_b128(from, there[g] + i * r_step, 0, 0));
+                }
+                return y;
+            };
+            v16u now = fetch(0);
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                v16u then{};
+                if (i + 1 < MB) then = fetch(i + 1);
+                float v[16];
+                value(i, v);
+                if (a.act.kind != CLDNN_HIP_ACT_NONE) act_apply<true>(v, a.act);
+                matmul_typed(a.res_type, [&](auto t) { matmul_add_row<decltype(t)>(now, v); });
+                if (a.act2.kind != CLDNN_HIP_ACT_NONE) act_apply<true>(v, a.act2);
+                store(i, v);
+                now = then;
+            }
+        } else {
+            act_choose(a.act.kind, [&](auto kind) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < MB; ++i) {
+                    float v[16];
+                    value(i, v);
+#pragma unroll
+                    for (int l = 0; l < 16; ++l) v[l] = act_one<decltype(kind)::value, true>(v[l], a.act.m, a.act.n);
+                    store(i, v);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            });
+        }
+        if (!more) break;
+        matmul_arrive<RUNS * MB>();  // the loads are older than the stores, of which there are so many
+    }
+}
 
 namespace {
 
@@ -17,7 +217,7 @@ struct MatmulS8Kernel {
 };
 enum { MM_256, MM_224, MM_192, MM_128, MM_64x128, MM_64, MM_32, MM_ANY_64, MM_ANY_32, MM_16 };
 const MatmulS8Kernel matmul_s8_kernels[] = {
-    {"matmul_s8_tile<256x256>", 256, 256, 8, 128 << 10}, {"matmul_s8_tile<224x256>", 224, 256, 8, 120 << 10}, {"matmul_s8_tile<192x256>", 192, 256, 8, 112 << 10},
+    {"matmul_s8_walk<256x256>", 256, 256, 8, 128 << 10}, {"matmul_s8_walk<224x256>", 224, 256, 8, 120 << 10}, {"matmul_s8_walk<192x256>", 192, 256, 8, 112 << 10},
     {"matmul_s8_tile<128x128>", 128, 128, 4, 64 << 10}, {"matmul_s8_tile<64x128>", 64, 128, 4, 72 << 10},
     {"matmul_s8_tile<64x64,k2>", 64, 64, 8, 128 << 10}, {"matmul_s8_tile<32x64,k4>", 32, 64, 8, 144 << 10},
     {"matmul_s8_split<64x64>", 64, 64, 4, 64 << 10}, {"matmul_s8_split<32x32>", 32, 32, 8, 32 << 10}, {"matmul_s8_split<16x16>", 16, 16, 8, 8 << 10},
@@ -27,6 +227,7 @@ struct MatmulS8Plan : OperatorPlan {
     MatmulS8Args a{};
     int kernel = 0;  // row of matmul_s8_kernels; the one for any strides where pointers are not aligned
     int any = 0;
+    int cus = 0;
     int pieces = 0;  // > 0: the operands are copied into rows of so many 16-byte pieces first
 };
 
@@ -89,7 +290,7 @@ std::unique_ptr<OperatorPlan> matmul_s8_plan(const cldnn_hip_engine_s& e, const 
     const auto mark = [](bool has) { return has ? (const float*)4 : nullptr; };
     a.a_scales = mark(d.a_scales != CLDNN_HIP_SCALES_NONE), a.w_scales = mark(d.weights_scales != CLDNN_HIP_SCALES_NONE);
     a.bias = mark(d.has_bias), a.residual = mark(res_size);
-    const int cus = e.props.multiProcessorCount;
+    const int cus = plan->cus = e.props.multiProcessorCount;
     const bool whole = d.k % 16 == 0 && a.a_pitch % 16 == 0 && a.w_pitch % 16 == 0 && std::max(a.a_pitch, a.w_pitch) < (1 << 22);
     plan->kernel = choose(d.m, d.n, whole, cus);
     plan->any = choose(d.m, d.n, false, cus);
@@ -101,7 +302,7 @@ std::unique_ptr<OperatorPlan> matmul_s8_plan(const cldnn_hip_engine_s& e, const 
     set_tiles(a, kernel);
     a.splits = 1;
     if (plan->kernel == MM_16 && a.tiles * 2 <= cus && d.k >= 16000) a.splits = std::min(cus / a.tiles, d.k / 4096);
-    info.launches = plan->pieces || a.splits > 1 ? 2 : 1, info.block = 64 * kernel.waves, info.grid = a.tiles * a.splits, info.lds_bytes = kernel.lds;
+    info.launches = plan->pieces || a.splits > 1 ? 2 : 1, info.block = 64 * kernel.waves, info.grid = plan->kernel <= MM_192 ? std::min(a.tiles, cus) : a.tiles * a.splits, info.lds_bytes = kernel.lds;
     if (plan->pieces) info.block = MATMUL_PACK_THREADS, info.grid = (int32_t)pack_blocks(*plan);
     info.workspace_bytes = ((int64_t)d.m + d.n) * plan->pieces * 16 + (a.splits > 1 ? (int64_t)a.splits * d.m * d.n * 4 : 0);
     info.ops = 2ll * d.m * d.n * d.k;
@@ -123,6 +324,9 @@ void matmul_s8_launch(hipStream_t s, const OperatorPlan& plan, void* workspace, 
     if (a.w_scales) check_aligned(w_scales, 4, "weights_scales"), a.w_scales = w_scales;
     if (a.bias) check_aligned(bias, 4, "bias"), a.bias = bias;
     if (a.residual) check_aligned(residual, float_size(a.res_type, ""), "residual"), a.residual = residual;
+    const int run = a.out_type == CLDNN_HIP_F32 ? 4 : 8, res_size = a.residual ? float_size(a.res_type, "") : 0;
+    const auto runs = [&](const void* p, int64_t pitch, int size) { return pitch % run == 0 && pitch <= MATMUL_S8_RUN_PITCH && ((uintptr_t)p & (std::min(16, run * size) - 1)) == 0; };
+    a.out_runs = a.n % run == 0 && runs(out, a.o_pitch, float_size(a.out_type, "")) && (!a.residual || runs(residual, a.r_pitch, res_size));
     const int8_t *xa = (const int8_t*)x, *wa = (const int8_t*)w;
     a.part = workspace;
     if (p.pieces) {
@@ -133,11 +337,16 @@ void matmul_s8_launch(hipStream_t s, const OperatorPlan& plan, void* workspace, 
     const int row = (((uintptr_t)xa | (uintptr_t)wa) & 15) == 0 ? p.kernel : p.any;
     const MatmulS8Kernel& kernel = matmul_s8_kernels[row];
     set_tiles(a, kernel);
-    const auto launch = [&](auto f) { hipLaunchKernelGGL(f, dim3(a.tiles, a.splits), dim3(64 * kernel.waves), 0, s, a, xa, wa, out); };
+    const auto launch = [&](auto f) { hipLaunchKernelGGL(f, dim3(row <= MM_192 && a.out_runs ? std::min(a.tiles, p.cus) : a.tiles, a.splits), dim3(64 * kernel.waves), 0, s, a, xa, wa, out); };
+    const auto large = [&](auto mb) {
+        constexpr int MB = decltype(mb)::value;
+        if (!a.out_runs) return launch(matmul_tile_kernel<int8_t, 2, 4, MB, 2, 1>);
+        with_float(a.out_type, [&](auto o) { launch(a.residual ? matmul_s8_walk_kernel<decltype(o), true, MB> : matmul_s8_walk_kernel<decltype(o), false, MB>); });
+    };
     switch (row) {
-    case MM_256: launch(matmul_tile_kernel<int8_t, 2, 4, 8, 2, 1>); break;
-    case MM_224: launch(matmul_tile_kernel<int8_t, 2, 4, 7, 2, 1>); break;
-    case MM_192: launch(matmul_tile_kernel<int8_t, 2, 4, 6, 2, 1>); break;
+    case MM_256: large(std::integral_constant<int, 8>()); break;
+    case MM_224: large(std::integral_constant<int, 7>()); break;
+    case MM_192: large(std::integral_constant<int, 6>()); break;
     case MM_128: launch(matmul_tile_kernel<int8_t, 2, 2, 4, 2, 1>); break;
     case MM_64x128: launch(matmul_tile_kernel<int8_t, 2, 2, 2, 3, 1>); break;
     case MM_64: launch(matmul_tile_kernel<int8_t, 4, 1, 1, 4, 2>); break;

@@ -24,7 +24,7 @@ struct QuantizePlan : OperatorPlan {
 __device__ __forceinline__ void quantize_values(const QuantizeArgs& a, const RowRaw& x, const RowRaw& gate, const float* factors, int c, float (&v)[8])
 {
     row_values(x, a.type, v);
-    act_apply(v, a.act);
+    act_apply<true>(v, a.act);
     if (a.gated) {
         float g[8];
         row_values(gate, a.type, g);
