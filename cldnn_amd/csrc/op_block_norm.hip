@@ -25,130 +25,114 @@ struct BlockNormPlan : OperatorPlan {
 
 __device__ inline int block_norm_size(int type) { return type == CLDNN_HIP_S8 ? 1 : type == CLDNN_HIP_F32 ? 4 : 2; }
 
-// Values of a row, zeros from C on, become their unit form; two slots of LDS.
-template <int LANES, int NV>
+// The values of a row, zeros where they are not the lane's, become their unit form; two slots of LDS.
+template <int LANES, int NV, int SURE>
 __device__ __forceinline__ void block_norm_unit(float (&v)[NV][8], int kind, int C, float epsilon, int lane, float (*slot)[LANES < 64 ? 1 : LANES / 64])
 {
     if (kind == CLDNN_HIP_TOKEN_NORM_NONE) return;
+    const auto each = [&](auto&& f) __attribute__((always_inline)) { row_each<LANES, NV, SURE>(lane, C, f); };
     if (kind == CLDNN_HIP_TOKEN_NORM_LAYER) {
         float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
+        each([&](int i, RowVector) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum += v[i][j];
+        });
         const float mean = row_sum<LANES>(sum, slot[0]) / (float)C;
+        each([&](int i, RowVector of) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = (lane + i * LANES) * 8 + j < C ? v[i][j] - mean : 0.0f;
+            for (int j = 0; j < 8; ++j) v[i][j] -= mean;
+            row_mask(of, C, v[i]);
+        });
     }
     float squares = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
+    each([&](int i, RowVector) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) squares = __builtin_fmaf(v[i][j], v[i][j], squares);
+    });
     const float factor = 1.0f / __builtin_sqrtf(row_sum<LANES>(squares, slot[1]) / (float)C + epsilon);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
+    each([&](int i, RowVector) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] *= factor;
+    });
 }
 
-template <int LANES, int NV>
-__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void block_norm_kernel(BlockNormArgs a, BlockNormPointers p)
+template <int LANES, int NV, int SURE>
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES, row_waves(NV)) void block_norm_kernel(BlockNormArgs a, BlockNormPointers p)
 {
     constexpr int THREADS = LANES < 256 ? 256 : LANES;
     __shared__ float slot[5][LANES < 64 ? 1 : LANES / 64];
-    const int lane = threadIdx.x & (LANES - 1);
+    const int lane = threadIdx.x & (LANES - 1), C = row_length<LANES, SURE>(a.C);
     const int64_t row = (int64_t)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
     if (row >= a.tokens) return;  // whole groups: nobody waits for them
     const int64_t image = a.per_image ? (uint32_t)row / (uint32_t)a.per_image : 0;
     const auto at = [](const void* base, int64_t elements, int type) { return (const char*)base + elements * block_norm_size(type); };
-    const char* x_row = at(p.x, row * a.x_pitch, a.x_type);
+    const auto each = [&](auto&& f) __attribute__((always_inline)) { row_each<LANES, NV, SURE>(lane, C, f); };
     const bool has_branch = a.branch_type != CLDNN_HIP_NO_TYPE;
-    RowRaw x[NV], branch[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) x[i] = row_load(x_row, a.x_type, (lane + i * LANES) * 8, a.C);
+    RowRaw<true> x[NV], branch[NV];
+    const char *x_row = at(p.x, row * a.x_pitch, a.x_type), *branch_row = at(p.branch, row * a.branch_pitch, a.branch_type);
+    if (has_branch) each([&](int i, RowVector of) { branch[i] = row_load<true>(branch_row, a.branch_type, of.c, C); });
+    each([&](int i, RowVector of) { x[i] = row_load<true>(x_row, a.x_type, of.c, C); });
     float v[NV][8];
+    const auto times = [&](int i, const float (&f)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] *= f[j];
+    };
+    const auto plus = [&](int i, const float (&f)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] += f[j];
+    };
+    // a vector of the image's row of gate, scale or shift
+    const auto modulation = [&](const void* base, int64_t pitch, int c, float (&f)[8]) { row_values(row_load<true>(at(base, image * pitch, a.mod_type), a.mod_type, c, C), a.mod_type, f); };
     if (has_branch) {
-        const char* branch_row = at(p.branch, row * a.branch_pitch, a.branch_type);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) branch[i] = row_load(branch_row, a.branch_type, (lane + i * LANES) * 8, a.C);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) row_values(branch[i], a.branch_type, v[i]);
-        block_norm_unit<LANES, NV>(v, a.post, a.C, a.post_epsilon, lane, slot);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (lane + i * LANES) * 8;
+        each([&](int i, RowVector of) { row_values(branch[i], a.branch_type, v[i]), row_mask(of, C, v[i]); });
+        block_norm_unit<LANES, NV, SURE>(v, a.post, C, a.post_epsilon, lane, slot);
+        each([&](int i, RowVector of) {
             float f[8];
-            if (p.post_weight) {
-                row_floats(p.post_weight, c, a.C, f);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] *= f[j];
-            }
-            if (p.post_bias) {
-                row_floats(p.post_bias, c, a.C, f);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] += f[j];
-            }
-            if (p.gate) {
-                row_values(row_load(at(p.gate, image * a.gate_pitch, a.mod_type), a.mod_type, c, a.C), a.mod_type, f);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] *= f[j];
-            }
+            if (p.post_weight) row_floats(p.post_weight, of.c, C, f), times(i, f);
+            if (p.post_bias) row_floats(p.post_bias, of.c, C, f), plus(i, f);
+            if (p.gate) modulation(p.gate, a.gate_pitch, of.c, f), times(i, f);
             row_values(x[i], a.x_type, f);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] = __builtin_fmaf(a.residual_scale, f[j], v[i][j]);
-            if (p.y && c < a.C) row_store((char*)p.y + row * a.y_pitch * block_norm_size(a.x_type), a.x_type, c, a.C, v[i]);
-        }
+            if (p.y) row_store((char*)p.y + row * a.y_pitch * block_norm_size(a.x_type), a.x_type, of, C, v[i]);
+            row_mask(of, C, v[i]);
+        });
     } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) row_values(x[i], a.x_type, v[i]);
+        each([&](int i, RowVector of) { row_values(x[i], a.x_type, v[i]), row_mask(of, C, v[i]); });
     }
     if (a.out_type == CLDNN_HIP_NO_TYPE) return;
-    block_norm_unit<LANES, NV>(v, a.norm, a.C, a.epsilon, lane, slot + 2);
-    uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (lane + i * LANES) * 8;
+    block_norm_unit<LANES, NV, SURE>(v, a.norm, C, a.epsilon, lane, slot + 2);
+    float most = 0.0f;
+    each([&](int i, RowVector of) {
         float f[8];
-        if (p.weight) {
-            row_floats(p.weight, c, a.C, f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] *= f[j];
-        }
-        if (p.bias) {
-            row_floats(p.bias, c, a.C, f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] += f[j];
-        }
+        if (p.weight) row_floats(p.weight, of.c, C, f), times(i, f);
+        if (p.bias) row_floats(p.bias, of.c, C, f), plus(i, f);
         if (p.scale) {
-            row_values(row_load(at(p.scale, image * a.scale_pitch, a.mod_type), a.mod_type, c, a.C), a.mod_type, f);
+            modulation(p.scale, a.scale_pitch, of.c, f);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] *= 1.0f + f[j];
         }
-        if (p.shift) {
-            row_values(row_load(at(p.shift, image * a.shift_pitch, a.mod_type), a.mod_type, c, a.C), a.mod_type, f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] += f[j];
-        }
+        if (p.shift) modulation(p.shift, a.shift_pitch, of.c, f), plus(i, f);
+        row_mask(of, C, v[i]);
         most = row_magnitude(v[i], most);
-    }
+    });
     if (a.out_type == CLDNN_HIP_S8) {
         const RowSteps steps = row_steps(row_most<LANES>(most, slot[4]));
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (lane + i * LANES) * 8;
-            if (c < a.C) row_store_s8((int8_t*)p.out + row * a.out_pitch + c, a.C - c, v[i], steps);
-        }
+        each([&](int i, RowVector of) { row_store_s8((int8_t*)p.out + row * a.out_pitch, of, C, v[i], steps); });
         if (lane == 0) p.out_scales[row] = steps.scale;
     } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (lane + i * LANES) * 8;
-            if (c < a.C) row_store((char*)p.out + row * a.out_pitch * block_norm_size(a.out_type), a.out_type, c, a.C, v[i]);
-        }
+        each([&](int i, RowVector of) { row_store((char*)p.out + row * a.out_pitch * block_norm_size(a.out_type), a.out_type, of, C, v[i]); });
     }
+}
+
+// The shape for rows of C values.  A wave to a row as long as three vectors a lane hold it, then more waves (us, bf16 with gate, scale and
+// shift: 20000 x 1500 54 by a wave, 60 by four; 12000 x 2048 49 and 41).
+template <typename F>
+static void block_norm_shape(int C, F&& f)
+{
+    (void)(try_row_shape<16, 1, 0>(C, f) || try_row_shape<16, 2, 1>(C, f) || try_row_shape<64, 1, 0>(C, f) || try_row_shape<64, 2, 1>(C, f) || try_row_shape<64, 3, 2>(C, f) ||
+           try_row_shape<256, 1, 0>(C, f) || try_row_shape<256, 2, 1>(C, f) || try_row_shape<256, 3, 2>(C, f) || try_row_shape<512, 2, 1>(C, f) || try_row_shape<512, 3, 2>(C, f) ||
+           try_row_shape<512, 4, 3>(C, f) || try_row_shape<512, 6, 4>(C, f) || try_row_shape<512, 8, 6>(C, f));
 }
 
 std::unique_ptr<OperatorPlan> block_norm_plan(const cldnn_hip_engine_s&, const cldnn_hip_block_norm_desc& d, cldnn_hip_operator_info& info)
@@ -176,7 +160,7 @@ std::unique_ptr<OperatorPlan> block_norm_plan(const cldnn_hip_engine_s&, const c
     };
     a.x_pitch = pitch(d.x_stride), a.branch_pitch = pitch(d.branch_stride), a.y_pitch = pitch(d.y_stride), a.out_pitch = pitch(d.out_stride);
     a.gate_pitch = pitch(d.gate_stride), a.scale_pitch = pitch(d.scale_stride), a.shift_pitch = pitch(d.shift_stride);
-    plan->shape = row_shape(d.features);
+    block_norm_shape(d.features, [&](auto lanes, auto vectors, auto) { plan->shape = {decltype(lanes)::value, decltype(vectors)::value}; });
     const int64_t blocks = plan->shape.blocks(d.tokens);
     check_grid(blocks, plan->shape.threads(), "block norm");
     info.launches = 1, info.grid = (int32_t)blocks, info.block = plan->shape.threads(), info.lds_bytes = plan->shape.lanes > 64 ? 5 * plan->shape.lanes / 64 * 4 : 0;
@@ -211,8 +195,9 @@ void block_norm_launch(hipStream_t s, const OperatorPlan& plan, const BlockNormP
     }
     check_aligned(given.post_weight, 4, "post_weight"), check_aligned(given.post_bias, 4, "post_bias"), check_aligned(given.weight, 4, "weight"), check_aligned(given.bias, 4, "bias");
     check_aligned(given.out_scales, 4, "out_scales");
-    with_row_shape(p.shape, [&](auto lanes, auto vectors) {
-        hipLaunchKernelGGL((block_norm_kernel<decltype(lanes)::value, decltype(vectors)::value>), dim3((unsigned)p.shape.blocks(a.tokens)), dim3(p.shape.threads()), 0, s, a, given);
+    block_norm_shape(a.C, [&](auto lanes, auto vectors, auto sure) {
+        hipLaunchKernelGGL((block_norm_kernel<decltype(lanes)::value, decltype(vectors)::value, decltype(sure)::value>), dim3((unsigned)p.shape.blocks(a.tokens)),
+                           dim3(p.shape.threads()), 0, s, a, given);
     });
     CHIP_CHECK(hipGetLastError());
 }

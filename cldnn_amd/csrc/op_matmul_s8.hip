@@ -214,10 +214,13 @@ struct MatmulS8Kernel {
     const char* name;
     int rows, features, waves;
     int lds;  // bytes: the stages of both operands, or the waves' sums
+    const char* walk;  // where the result is whole runs: the kernel that goes through several tiles, which has the scales in LDS besides
+    int walk_lds() const { return lds + 4 * (rows + 2 * features); }
 };
 enum { MM_256, MM_224, MM_192, MM_128, MM_64x128, MM_64, MM_32, MM_ANY_64, MM_ANY_32, MM_16 };
 const MatmulS8Kernel matmul_s8_kernels[] = {
-    {"matmul_s8_walk<256x256>", 256, 256, 8, 128 << 10}, {"matmul_s8_walk<224x256>", 224, 256, 8, 120 << 10}, {"matmul_s8_walk<192x256>", 192, 256, 8, 112 << 10},
+    {"matmul_s8_tile<256x256>", 256, 256, 8, 128 << 10, "matmul_s8_walk<256x256>"}, {"matmul_s8_tile<224x256>", 224, 256, 8, 120 << 10, "matmul_s8_walk<224x256>"},
+    {"matmul_s8_tile<192x256>", 192, 256, 8, 112 << 10, "matmul_s8_walk<192x256>"},
     {"matmul_s8_tile<128x128>", 128, 128, 4, 64 << 10}, {"matmul_s8_tile<64x128>", 64, 128, 4, 72 << 10},
     {"matmul_s8_tile<64x64,k2>", 64, 64, 8, 128 << 10}, {"matmul_s8_tile<32x64,k4>", 32, 64, 8, 144 << 10},
     {"matmul_s8_split<64x64>", 64, 64, 4, 64 << 10}, {"matmul_s8_split<32x32>", 32, 32, 8, 32 << 10}, {"matmul_s8_split<16x16>", 16, 16, 8, 8 << 10},
@@ -228,6 +231,7 @@ struct MatmulS8Plan : OperatorPlan {
     int kernel = 0;  // row of matmul_s8_kernels; the one for any strides where pointers are not aligned
     int any = 0;
     int cus = 0;
+    bool runs = false;  // sizes and strides allow whole runs of results
     int pieces = 0;  // > 0: the operands are copied into rows of so many 16-byte pieces first
 };
 
@@ -251,6 +255,8 @@ int choose(int m, int n, bool whole, int cus)
     if (tiles(MM_64) * 4 >= cus * 3) return MM_64;
     return MM_32;
 }
+
+int matmul_s8_run(const MatmulS8Args& a) { return a.out_type == CLDNN_HIP_F32 ? 4 : 8; }
 
 void set_tiles(MatmulS8Args& a, const MatmulS8Kernel& k)
 {
@@ -290,6 +296,8 @@ std::unique_ptr<OperatorPlan> matmul_s8_plan(const cldnn_hip_engine_s& e, const 
     const auto mark = [](bool has) { return has ? (const float*)4 : nullptr; };
     a.a_scales = mark(d.a_scales != CLDNN_HIP_SCALES_NONE), a.w_scales = mark(d.weights_scales != CLDNN_HIP_SCALES_NONE);
     a.bias = mark(d.has_bias), a.residual = mark(res_size);
+    const auto runs = [&](int64_t pitch) { return pitch % matmul_s8_run(a) == 0 && pitch <= MATMUL_S8_RUN_PITCH; };
+    plan->runs = a.n % matmul_s8_run(a) == 0 && runs(a.o_pitch) && (!a.residual || runs(a.r_pitch));
     const int cus = plan->cus = e.props.multiProcessorCount;
     const bool whole = d.k % 16 == 0 && a.a_pitch % 16 == 0 && a.w_pitch % 16 == 0 && std::max(a.a_pitch, a.w_pitch) < (1 << 22);
     plan->kernel = choose(d.m, d.n, whole, cus);
@@ -302,14 +310,16 @@ std::unique_ptr<OperatorPlan> matmul_s8_plan(const cldnn_hip_engine_s& e, const 
     set_tiles(a, kernel);
     a.splits = 1;
     if (plan->kernel == MM_16 && a.tiles * 2 <= cus && d.k >= 16000) a.splits = std::min(cus / a.tiles, d.k / 4096);
-    info.launches = plan->pieces || a.splits > 1 ? 2 : 1, info.block = 64 * kernel.waves, info.grid = plan->kernel <= MM_192 ? std::min(a.tiles, cus) : a.tiles * a.splits, info.lds_bytes = kernel.lds;
+    info.launches = plan->pieces || a.splits > 1 ? 2 : 1, info.block = 64 * kernel.waves, info.grid = a.tiles * a.splits, info.lds_bytes = kernel.lds;
+    const bool walk = kernel.walk && plan->runs;
+    if (walk) info.grid = std::min(a.tiles, cus), info.lds_bytes = kernel.walk_lds();
     if (plan->pieces) info.block = MATMUL_PACK_THREADS, info.grid = (int32_t)pack_blocks(*plan);
     info.workspace_bytes = ((int64_t)d.m + d.n) * plan->pieces * 16 + (a.splits > 1 ? (int64_t)a.splits * d.m * d.n * 4 : 0);
     info.ops = 2ll * d.m * d.n * d.k;
     const auto scales = [](int kind, int64_t rows) { return kind == CLDNN_HIP_SCALES_EACH ? 4 * rows : kind == CLDNN_HIP_SCALES_ONE ? 4 : 0; };
     info.bytes = (int64_t)d.m * d.k + (int64_t)d.n * d.k + scales(d.a_scales, d.m) + scales(d.weights_scales, d.n) + (d.has_bias ? 4ll * d.n : 0) +
                  (int64_t)d.m * d.n * (out_size + res_size);
-    snprintf(info.kernel_name, sizeof info.kernel_name, "%s%s%s", plan->pieces ? "matmul_pack + " : "", kernel.name, a.splits > 1 ? " + matmul_join" : "");
+    snprintf(info.kernel_name, sizeof info.kernel_name, "%s%s%s", plan->pieces ? "matmul_pack + " : "", walk ? kernel.walk : kernel.name, a.splits > 1 ? " + matmul_join" : "");
     return plan;
 }
 
@@ -324,9 +334,8 @@ void matmul_s8_launch(hipStream_t s, const OperatorPlan& plan, void* workspace, 
     if (a.w_scales) check_aligned(w_scales, 4, "weights_scales"), a.w_scales = w_scales;
     if (a.bias) check_aligned(bias, 4, "bias"), a.bias = bias;
     if (a.residual) check_aligned(residual, float_size(a.res_type, ""), "residual"), a.residual = residual;
-    const int run = a.out_type == CLDNN_HIP_F32 ? 4 : 8, res_size = a.residual ? float_size(a.res_type, "") : 0;
-    const auto runs = [&](const void* p, int64_t pitch, int size) { return pitch % run == 0 && pitch <= MATMUL_S8_RUN_PITCH && ((uintptr_t)p & (std::min(16, run * size) - 1)) == 0; };
-    a.out_runs = a.n % run == 0 && runs(out, a.o_pitch, float_size(a.out_type, "")) && (!a.residual || runs(residual, a.r_pitch, res_size));
+    const auto whole = [&](const void* p, int type) { return ((uintptr_t)p & (std::min(16, matmul_s8_run(a) * float_size(type, "")) - 1)) == 0; };
+    a.out_runs = p.runs && whole(out, a.out_type) && (!a.residual || whole(residual, a.res_type));
     const int8_t *xa = (const int8_t*)x, *wa = (const int8_t*)w;
     a.part = workspace;
     if (p.pieces) {
@@ -337,7 +346,7 @@ void matmul_s8_launch(hipStream_t s, const OperatorPlan& plan, void* workspace, 
     const int row = (((uintptr_t)xa | (uintptr_t)wa) & 15) == 0 ? p.kernel : p.any;
     const MatmulS8Kernel& kernel = matmul_s8_kernels[row];
     set_tiles(a, kernel);
-    const auto launch = [&](auto f) { hipLaunchKernelGGL(f, dim3(row <= MM_192 && a.out_runs ? std::min(a.tiles, p.cus) : a.tiles, a.splits), dim3(64 * kernel.waves), 0, s, a, xa, wa, out); };
+    const auto launch = [&](auto f) { hipLaunchKernelGGL(f, dim3(kernel.walk && a.out_runs ? std::min(a.tiles, p.cus) : a.tiles, a.splits), dim3(64 * kernel.waves), 0, s, a, xa, wa, out); };
     const auto large = [&](auto mb) {
         constexpr int MB = decltype(mb)::value;
         if (!a.out_runs) return launch(matmul_tile_kernel<int8_t, 2, 4, MB, 2, 1>);

@@ -1,4 +1,6 @@
-// Rows held in registers: a row belongs to a group of LANES threads, lane l of which has the vectors l, l + LANES, .. of 8 values.
+// Rows held in registers: a row belongs to a group of LANES threads, lane l of which has the vectors l, l + LANES, .. of 8 values.  The
+// last vector of a row that is no whole vectors lies over the one before it, so that all loads are whole; the values that it shares
+// are the other lane's (RowVector::from).  (One element at a time, the last vectors of 25088 x 1100 doubled the time of a norm.)
 // What the operators that go over rows share: loads and stores of any float type at any element's address, sums and maxima over a row,
 // quantised rows.
 #pragma once
@@ -10,47 +12,90 @@ namespace chip {
 // (1024 threads with 4 vectors each, in 128 registers, keep some in scratch memory).
 constexpr int ROW_MOST = 8 * 512 * 8;
 
-// 8 values as they lie in memory: f32 takes both, the 16-bit types the first
+// Waves of a SIMD that a kernel with NV vectors a lane leaves registers for: what covers a row's trips to memory is other rows.
+constexpr int row_waves(int NV) { return NV == 1 ? 7 : NV == 2 ? 6 : NV == 3 ? 4 : NV == 4 ? 3 : 2; }
+
+// The vector of a lane: values c .. c + 7 of the row, of which those from `from` on, and below C, are the lane's.
+struct RowVector {
+    int c, from;
+    __device__ __forceinline__ bool whole(int C) const { return from == 0 && C >= 8; }
+    __device__ __forceinline__ bool has(int i, int C) const { return i >= from && c + i < C; }
+};
+
+// f(i, vector) for the vectors of a lane.  The first SURE of them are whole for every lane.  One behind the row is the row's last
+// vector, with nothing in it that is the lane's: the program has no branch around what is done with it.
+template <int LANES, int NV, int SURE, typename F>
+__device__ __forceinline__ void row_each(int lane, int C, F&& f)
+{
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (lane + i * LANES) * 8, at = i < SURE ? c : min(c, max(C - 8, 0));
+        f(i, RowVector{at, c - at});
+    }
+}
+
+// the length of a row, of which the compiler may know that longer shapes have at least a vector
+template <int LANES, int SURE>
+__device__ __forceinline__ int row_length(int C)
+{
+    if constexpr (LANES > 16 || SURE > 0) __builtin_assume(C > 128);
+    return C;
+}
+
+// what is not the lane's becomes zero
+__device__ __forceinline__ void row_mask(const RowVector& of, int C, float (&v)[8])
+{
+    if (!of.whole(C))
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = of.has(i, C) ? v[i] : 0.0f;
+}
+
+// 8 values as they lie in memory: f32 takes both, the 16-bit types the first.  WIDE: it may be f32.
+template <bool WIDE>
 struct RowRaw {
     v4i a, b;
 };
+template <>
+struct RowRaw<false> {
+    v4i a;
+};
 
-// The values c .. c + 7 of a row; zeros from C on.
-__device__ __forceinline__ RowRaw row_load(const void* row, int type, int c, int C)
+// The values c .. c + 7 of a row, which is shorter than that if it has less than 8: zeros then.
+template <bool WIDE>
+__device__ __forceinline__ RowRaw<WIDE> row_load(const void* row, int type, int c, int C)
 {
     typedef v4i any4 __attribute__((aligned(4)));
-    RowRaw x;
-    if (type == CLDNN_HIP_F32) {
-        const float* p = (const float*)row + c;
-        if (c + 8 <= C) x.a = ((const any4*)p)[0], x.b = ((const any4*)p)[1];
-        else {
-            x.a = x.b = v4i{0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (c + i < C) x.a[i] = __builtin_bit_cast(int, p[i]);
-                if (c + 4 + i < C) x.b[i] = __builtin_bit_cast(int, p[4 + i]);
+    RowRaw<WIDE> x;
+    if constexpr (WIDE)
+        if (type == CLDNN_HIP_F32) {
+            const float* p = (const float*)row + c;
+            if (C >= 8) x.a = ((const any4*)p)[0], x.b = ((const any4*)p)[1];
+            else {
+                x.a = x.b = v4i{0, 0, 0, 0};
+                for (int i = 0; i < C; ++i) (i < 4 ? x.a : x.b)[i & 3] = __builtin_bit_cast(int, p[i]);
             }
+            return x;
         }
-    } else {
-        const uint16_t* p = (const uint16_t*)row + c;
-        if (c + 8 <= C) x.a = *(const v4i_any*)p;
-        else {
-            x.a = v4i{0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c + i < C) x.a[i / 2] |= (int)p[i] << (16 * (i & 1));
-        }
+    const uint16_t* p = (const uint16_t*)row + c;
+    if (C >= 8) x.a = *(const v4i_any*)p;
+    else {
+        x.a = v4i{0, 0, 0, 0};
+        for (int i = 0; i < C; ++i) x.a[i / 2] |= (int)p[i] << (16 * (i & 1));
     }
     return x;
 }
 
-__device__ __forceinline__ void row_values(const RowRaw& x, int type, float (&v)[8])
+template <bool WIDE>
+__device__ __forceinline__ void row_values(const RowRaw<WIDE>& x, int type, float (&v)[8])
 {
-    if (type == CLDNN_HIP_F32) {
-        const v4f a = __builtin_bit_cast(v4f, x.a), b = __builtin_bit_cast(v4f, x.b);
+    if constexpr (WIDE)
+        if (type == CLDNN_HIP_F32) {
+            const v4f a = __builtin_bit_cast(v4f, x.a), b = __builtin_bit_cast(v4f, x.b);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
-    } else if (type == CLDNN_HIP_F16) {
+            for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+            return;
+        }
+    if (type == CLDNN_HIP_F16) {
         const v8h h = __builtin_bit_cast(v8h, x.a);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
@@ -61,15 +106,16 @@ __device__ __forceinline__ void row_values(const RowRaw& x, int type, float (&v)
     }
 }
 
-__device__ __forceinline__ void row_floats(const float* row, int c, int C, float (&v)[8]) { row_values(row_load(row, CLDNN_HIP_F32, c, C), CLDNN_HIP_F32, v); }
+__device__ __forceinline__ void row_floats(const float* row, int c, int C, float (&v)[8]) { row_values(row_load<true>(row, CLDNN_HIP_F32, c, C), CLDNN_HIP_F32, v); }
 
 template <typename T>
-__device__ __forceinline__ void row_store_as(T* p, int valid, const float (&v)[8])
+__device__ __forceinline__ void row_store_as(T* row, const RowVector& of, int C, const float (&v)[8])
 {
     typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
     typedef T any __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
     constexpr int W = 16 / sizeof(T);
-    if (valid >= 8) {
+    T* p = row + of.c;
+    if (of.whole(C)) {
 #pragma unroll
         for (int j = 0; j < 8 / W; ++j) {
             vec x;
@@ -77,19 +123,19 @@ __device__ __forceinline__ void row_store_as(T* p, int valid, const float (&v)[8
             for (int i = 0; i < W; ++i) x[i] = (T)v[W * j + i];
             ((any*)p)[j] = x;
         }
-    } else {
+    } else if (of.from < 8) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < valid) p[i] = (T)v[i];
+            if (of.has(i, C)) p[i] = (T)v[i];
     }
 }
 
 // rounded once, to the type
-__device__ __forceinline__ void row_store(void* row, int type, int c, int C, const float (&v)[8])
+__device__ __forceinline__ void row_store(void* row, int type, const RowVector& of, int C, const float (&v)[8])
 {
-    if (type == CLDNN_HIP_F32) row_store_as((float*)row + c, C - c, v);
-    else if (type == CLDNN_HIP_F16) row_store_as((_Float16*)row + c, C - c, v);
-    else row_store_as((__bf16*)row + c, C - c, v);
+    if (type == CLDNN_HIP_F32) row_store_as((float*)row, of, C, v);
+    else if (type == CLDNN_HIP_F16) row_store_as((_Float16*)row, of, C, v);
+    else row_store_as((__bf16*)row, of, C, v);
 }
 
 // ----------------------------------------------------------------------------- over a row
@@ -123,20 +169,17 @@ __device__ __forceinline__ float row_sum(float v, float* slot)
     return row_all<LANES>(v, slot, [](float a, float b) { return a + b; });
 }
 
-// magnitudes as the bits of a float, which compare like whole numbers: NaN is above infinity
+// the largest magnitude; NaN where a value is NaN
 template <int LANES>
-__device__ __forceinline__ uint32_t row_most(uint32_t v, float* slot)
+__device__ __forceinline__ float row_most(float v, float* slot)
 {
-    return row_all<LANES>(v, (uint32_t*)slot, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+    return row_all<LANES>(v, slot, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
 }
 
-__device__ __forceinline__ uint32_t row_magnitude(const float (&v)[8], uint32_t most)
+__device__ __forceinline__ float row_magnitude(const float (&v)[8], float most)
 {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t m = __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu;
-        most = m > most ? m : most;
-    }
+    for (int i = 0; i < 8; ++i) most = __builtin_elementwise_maximum(most, __builtin_fabsf(v[i]));
     return most;
 }
 
@@ -146,10 +189,9 @@ struct RowSteps {
     bool bad;  // a value that is not finite
 };
 
-__device__ __forceinline__ RowSteps row_steps(uint32_t most_bits)
+__device__ __forceinline__ RowSteps row_steps(float most)
 {
-    const float most = __builtin_bit_cast(float, most_bits);
-    RowSteps s{0.0f, 0.0f, most_bits >= 0x7f800000u};
+    RowSteps s{0.0f, 0.0f, !(most < __builtin_inff())};
     if (s.bad) s.scale = __builtin_nanf("");
     else if (most >= 0x1p-120f) s.inverse = 127.0f / most, s.scale = most / 127.0f;  // 127 * 2^120 is finite
     return s;
@@ -157,7 +199,7 @@ __device__ __forceinline__ RowSteps row_steps(uint32_t most_bits)
 
 // Rounds by adding 3 * 2^22: what is left in the low byte is the whole number in two's complement.  |v * inverse| is 127 and a rounding
 // at most.
-__device__ __forceinline__ void row_store_s8(int8_t* p, int valid, const float (&v)[8], const RowSteps& s)
+__device__ __forceinline__ void row_store_s8(int8_t* row, const RowVector& of, int C, const float (&v)[8], const RowSteps& s)
 {
 #pragma clang fp contract(off)
     uint32_t bits[8];
@@ -173,11 +215,12 @@ __device__ __forceinline__ void row_store_s8(int8_t* p, int valid, const float (
         q[j] = s.bad ? 0 : (int)(lo | hi << 16);
     }
     typedef v2i any __attribute__((aligned(1)));
-    if (valid >= 8) *(any*)p = q;
-    else {
+    int8_t* p = row + of.c;
+    if (of.whole(C)) *(any*)p = q;
+    else if (of.from < 8) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < valid) p[i] = (int8_t)((uint32_t)q[i / 4] >> (8 * (i & 3)));
+            if (of.has(i, C)) p[i] = (int8_t)((uint32_t)q[i / 4] >> (8 * (i & 3)));
     }
 }
 
@@ -189,38 +232,14 @@ struct RowShape {
     int64_t blocks(int64_t all) const { return (all + rows() - 1) / rows(); }
 };
 
-// rows of C values, at most ROW_MOST
-inline RowShape row_shape(int C)
+// f(lanes, vectors, SURE as constants) if that shape holds a row of C values.  An operator tries its shapes in order; SURE is what the one
+// before leaves for sure.
+template <int LANES, int NV, int SURE, typename F>
+bool try_row_shape(int C, F&& f)
 {
-    const int vectors = (C + 7) / 8;
-    for (const RowShape s : {RowShape{16, 1}, RowShape{64, 1}, RowShape{64, 2}, RowShape{64, 4}, RowShape{256, 2}, RowShape{256, 4}, RowShape{512, 4}})
-        if (vectors <= s.lanes * s.vectors) return s;
-    return RowShape{512, 8};
-}
-
-// f(lanes, vectors as constants)
-template <typename F>
-void with_row_shape(const RowShape& s, F&& f)
-{
-    const auto c = [&](auto lanes, auto vectors) { f(lanes, vectors); };
-    typedef std::integral_constant<int, 16> L16;
-    typedef std::integral_constant<int, 64> L64;
-    typedef std::integral_constant<int, 256> L256;
-    typedef std::integral_constant<int, 512> L512;
-    typedef std::integral_constant<int, 1> V1;
-    typedef std::integral_constant<int, 2> V2;
-    typedef std::integral_constant<int, 4> V4;
-    typedef std::integral_constant<int, 8> V8;
-    switch (s.lanes * 8 + s.vectors) {
-    case 16 * 8 + 1: return c(L16(), V1());
-    case 64 * 8 + 1: return c(L64(), V1());
-    case 64 * 8 + 2: return c(L64(), V2());
-    case 64 * 8 + 4: return c(L64(), V4());
-    case 256 * 8 + 2: return c(L256(), V2());
-    case 256 * 8 + 4: return c(L256(), V4());
-    case 512 * 8 + 4: return c(L512(), V4());
-    default: return c(L512(), V8());
-    }
+    if ((C + 7) / 8 > LANES * NV) return false;
+    f(std::integral_constant<int, LANES>(), std::integral_constant<int, NV>(), std::integral_constant<int, SURE>());
+    return true;
 }
 
 }  // namespace chip

@@ -145,7 +145,7 @@ def test_scales_that_are_no_number_stay_in_their_rows(eng, size):
 
 
 KERNELS = [
-    ((4090, 4093, 144), "walk<256x256>"), ((7160, 2040, 272), "walk<224x256>"), ((6130, 2046, 64), "walk<192x256>"), ((3100, 1537, 208), "tile<128x128>"),
+    ((4090, 4093, 144), "tile<256x256>"), ((7160, 2042, 272), "tile<224x256>"), ((6130, 2046, 64), "tile<192x256>"), ((4090, 4092, 144), "walk<256x256>"), ((7160, 2040, 272), "walk<224x256>"), ((6130, 2044, 64), "walk<192x256>"), ((3100, 1537, 208), "tile<128x128>"),
     ((1601, 1000, 112), "tile<64x128>"), ((1001, 1000, 272), "tile<64x64,k2>"), ((190, 2000, 528), "tile<32x64,k4>"), ((30, 1000, 1000), "split<16x16>"),
     ((7, 250, 18000), "split<16x16> + matmul_join"), ((1, 31, 16383), "split<16x16> + matmul_join"), ((20, 65, 18200), "split<16x16> + matmul_join"),
     ((1001, 1000, 255), "tile<64x64,k2>"), ((600, 500, 63), "split<32x32>"), ((1601, 1400, 61), "split<64x64>"), ((3101, 1500, 263), "tile<64x128>"), ((3101, 1700, 263), "tile<128x128>")]
@@ -158,11 +158,13 @@ def test_every_kernel(eng, size, kernel):
     assert kernel in info(op) and op.info().launches == (2 if k % 16 and ("tile" in kernel or "walk" in kernel) or "join" in kernel else 1), info(op)
     op.close()
     half = "f16" if m % 2 else "bf16"
-    if "walk" in kernel:  # results that are whole runs and others, several tiles to a workgroup, each with its last rows and features
-        for columns in (n // 8 * 8, n // 8 * 8 - 4):
-            check(eng, m, columns, k, out=half, act="gelu")
-            check(eng, m, columns, k, out="f32", act="silu", residual=half, act2="relu")
-            check(eng, m, columns, k, out=half, residual="f32", spare=(0, 0, 8, 8), a_scales="one", w_scales=None)
+    if "walk" in kernel:  # several tiles to a workgroup, each with its last rows and features; f32 results of runs of 4, others of 8
+        check(eng, m, n, k, out="f32", act="gelu", bias=False)
+        check(eng, m, n, k, out="f32", act="silu", residual=half, act2="relu")
+        check(eng, m, n // 8 * 8, k, out=half, act="gelu")
+        check(eng, m, n // 8 * 8, k, out=half, residual="f32", spare=(0, 0, 8, 8), a_scales="one", w_scales=None, in_place=False)
+        check(eng, m, n // 8 * 8, k, out=half, act="relu", residual=half, in_place=True)
+        check(eng, m, n // 8 * 8, k, out=half, act="relu", offsets=(0, 0, 1, 0))
     check(eng, m, n, k, out=half, act="gelu", residual=half)
     if "join" in kernel:
         check(eng, m, n, k, out="f32", act="relu", residual="f32", act2="silu", in_place=True)

@@ -88,7 +88,7 @@ def infos_describe_the_launches(directory):
         made.append((ops_s8.Quantize(e, ops_s8.quantize_desc(rows, features, "f16")), 4))
         if features <= 32768:
             made.append((ops_s8.BlockNorm(e, ops_s8.block_norm_desc(rows, features, "f32", branch_dtype="f16", out_dtype="s8")), 12))
-    for m, n, k in ((4090, 4093, 144), (7160, 2040, 272), (6130, 2046, 64), (3100, 1537, 208), (1601, 1000, 112), (1001, 1000, 272), (190, 2000, 528), (30, 1000, 1000), (7, 250, 30000),
+    for m, n, k in ((4090, 4093, 144), (7160, 2042, 272), (6130, 2046, 64), (4090, 4092, 144), (7160, 2040, 272), (6130, 2044, 64), (3100, 1537, 208), (1601, 1000, 112), (1001, 1000, 272), (190, 2000, 528), (30, 1000, 1000), (7, 250, 30000),
                     (600, 500, 63), (1601, 1400, 61), (1001, 1000, 255), (1, 1, 1)):
         made.append((ops_s8.MatmulS8(e, ops_s8.matmul_s8_desc(m, n, k)), 7))
     hip_path = hip.LIB_PATH
@@ -106,6 +106,7 @@ def infos_describe_the_launches(directory):
         for part in ("matmul_pack", "matmul_join", "quantize", "block_norm"):
             assert (part in name) == any(part in l[1] for l in found), "%s: %r" % (name, [l[1] for l in found])
         assert ("split" in name) == any("matmul_split" in l[1] for l in found) and ("tile" in name) == any("matmul_tile" in l[1] for l in found)
+        assert ("walk" in name) == any("matmul_s8_walk" in l[1] for l in found)
 
 
 @pytest.mark.skipif(not os.path.exists(host.READELF), reason="needs the kernels' metadata")
