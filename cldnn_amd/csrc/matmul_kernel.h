@@ -60,6 +60,11 @@ __device__ inline v4i matmul_load(const T* row, int k, int K)
     constexpr int E = MatmulType<T>::E;
     typedef typename MatmulType<T>::Any any;
     if (k + E <= K) return *(const any*)(row + k);
+    if constexpr (E == 16)
+        if (K >= E) {  // the row's last piece, moved (one value at a time: 13.7 us instead of 6.8 for 1000 x 127 -> 1000)
+            const unsigned __int128 last = __builtin_bit_cast(unsigned __int128, (v4i)*(const any*)(row + K - E));
+            return __builtin_bit_cast(v4i, k < K ? last >> (8 * (k + E - K)) : (unsigned __int128)0);
+        }
     typedef std::conditional_t<E == 8, short, signed char> I;
     typedef I vE __attribute__((ext_vector_type(E)));
     union {

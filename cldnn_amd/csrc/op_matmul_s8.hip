@@ -7,7 +7,10 @@ namespace chip {
 
 constexpr int MATMUL_S8_MOST_K = 131071;  // 128 * 128 of each fit 31 bits
 constexpr int64_t MATMUL_S8_RUN_PITCH = 1 << 20;  // 256 rows of it in f32 are within a buffer's reach
-constexpr int64_t MATMUL_S8_PACK = 200ll << 20;  // products from which unaligned operands are copied
+// Products from which unaligned operands are copied: a launch and two trips of the operands against the kernels for any rows (us, without
+// the copy and with it: 1000 x 401 -> 400 7.1 and 7.9, 1000 x 255 -> 1000 9.2 and 8.1, 1500 x 255 -> 1000 13.0 and 8.4, 20000 x 84 -> 400
+// 27 and 12).
+constexpr int64_t MATMUL_S8_PACK = 200ll << 20;
 
 // Large products: 32 MB rows x 256 features at a time to a workgroup of 2 x 4 waves, which goes through tiles i, i + grid, .. of the result.
 // The main loop is that of matmul_tile_kernel<2, 4, MB>, whose comment says how the halves of the waves take turns; what is different
@@ -239,21 +242,37 @@ int64_t pack_blocks(const MatmulS8Plan& p) { return (((int64_t)p.a.m + p.a.n) * 
 
 int64_t count(int m, int n, const MatmulS8Kernel& k) { return (int64_t)((m + k.rows - 1) / k.rows) * ((n + k.features - 1) / k.features); }
 
+// What a kernel takes in us behind a launch: for each round that its tiles need on the chip, base + step * K, measured over 324 sizes of 1 to
+// 25088 rows, 96 to 8192 features and K of 256 to 16384 (f16 results).  Of two workgroups to a CU a full round has both, and a last
+// one of at most one to a CU has the `one` figures.  The kernel with the least sum was the best or within 6 % of it.
+struct MatmulS8Time {
+    int kernel, on_cu;  // workgroups to a CU
+    double base, step, one_base, one_step;
+};
+const MatmulS8Time matmul_s8_times[] = {
+    {MM_256, 1, 7.8, 0.0092}, {MM_224, 1, 7.0, 0.0086}, {MM_192, 1, 6.3, 0.0078}, {MM_128, 2, 6.0, 0.0062, 4.5, 0.0045},
+    {MM_64x128, 2, 4.3, 0.0038, 3.9, 0.0027}, {MM_64, 1, 3.7, 0.0015}, {MM_32, 1, 3.7, 0.0011},
+};
+
 // whole: rows of 16-byte pieces, which the direct loads into LDS need
-int choose(int m, int n, bool whole, int cus)
+int choose(int m, int n, int k, bool whole, int cus)
 {
     const auto tiles = [&](int row) { return count(m, n, matmul_s8_kernels[row]); };
-    const auto rounds = [&](int row) { return (tiles(row) + cus - 1) / cus; };
-    if (tiles(MM_16) * 4 <= cus * 5) return MM_16;
+    // Few tiles of any size: the smallest, whose eight waves split K.  (us, against 32 x 64 tiles: 32 x 256 -> 4096, 512 of them, 4.4 and 6.0,
+    // 32 x 1024 -> 4096 5.3 and 6.5, 1 x 4096 -> 8192 8.6 and 10.5; every one reads all of its rows, so not many with a long K: 784 x 4096
+    // -> 96, 294 of them, 10.5 and 9.0)
+    const int64_t few = tiles(MM_16);
+    if (few <= (k <= 512 ? 3 * cus : k <= 1024 || m <= 16 ? 2 * cus : k <= 2048 || m <= 64 ? cus * 5 / 4 : cus)) return MM_16;
     if (!whole) return tiles(MM_ANY_64) >= cus ? MM_ANY_64 : MM_ANY_32;
-    if (tiles(MM_128) * 4 >= cus * 5) {
-        const int kernel[] = {MM_256, MM_224, MM_192, MM_128};
-        const double time[] = {rounds(MM_256) * 256.0, rounds(MM_224) * 224 * 1.04, rounds(MM_192) * 192 * 1.12, rounds(MM_128) * 64 * 1.22};
-        return kernel[std::min_element(time, time + 4) - time];
+    int best = MM_32;
+    double least = 1e30;
+    for (const MatmulS8Time& t : matmul_s8_times) {
+        const int64_t all = tiles(t.kernel), full = all / (t.on_cu * cus), rest = all - full * t.on_cu * cus;
+        const double round = t.base + t.step * k, last = t.on_cu > 1 && rest <= cus ? t.one_base + t.one_step * k : round;
+        const double time = full * round + (rest ? last : 0.0);
+        if (time < least) least = time, best = t.kernel;
     }
-    if (tiles(MM_64x128) * 4 >= cus * 3) return MM_64x128;
-    if (tiles(MM_64) * 4 >= cus * 3) return MM_64;
-    return MM_32;
+    return best;
 }
 
 int matmul_s8_run(const MatmulS8Args& a) { return a.out_type == CLDNN_HIP_F32 ? 4 : 8; }
@@ -300,16 +319,19 @@ std::unique_ptr<OperatorPlan> matmul_s8_plan(const cldnn_hip_engine_s& e, const 
     plan->runs = a.n % matmul_s8_run(a) == 0 && runs(a.o_pitch) && (!a.residual || runs(a.r_pitch));
     const int cus = plan->cus = e.props.multiProcessorCount;
     const bool whole = d.k % 16 == 0 && a.a_pitch % 16 == 0 && a.w_pitch % 16 == 0 && std::max(a.a_pitch, a.w_pitch) < (1 << 22);
-    plan->kernel = choose(d.m, d.n, whole, cus);
-    plan->any = choose(d.m, d.n, false, cus);
+    plan->kernel = choose(d.m, d.n, d.k, whole, cus);
+    plan->any = choose(d.m, d.n, d.k, false, cus);
     if (!whole && plan->any != MM_16 && (double)d.m * d.n * d.k >= MATMUL_S8_PACK && ((int64_t)d.m + d.n) * ((d.k + 15) / 16) < (1ll << 32) - MATMUL_PACK_THREADS) {
         plan->pieces = (d.k + 15) / 16;
-        plan->kernel = choose(d.m, d.n, true, cus);
+        plan->kernel = choose(d.m, d.n, d.k, true, cus);
     }
     const MatmulS8Kernel& kernel = matmul_s8_kernels[plan->kernel];
     set_tiles(a, kernel);
+    // The smallest tiles that leave half of the chip idle over a long K: workgroups that take 8192 of it each, a run of loads of their waves,
+    // for the price of a second launch (us, one workgroup and several: 16 x 25088 -> 1000 24.9 and 13.8, 16 x 16384 -> 1000 17.0 and 13.1,
+    // 1 x 16384 -> 500 11.6 and 9.9; 1 x 12288 -> 500 9.5 and 9.8; more and shorter parts gain nothing).
     a.splits = 1;
-    if (plan->kernel == MM_16 && a.tiles * 2 <= cus && d.k >= 16000) a.splits = std::min(cus / a.tiles, d.k / 4096);
+    if (plan->kernel == MM_16 && a.tiles * 2 <= cus && d.k > 12288) a.splits = std::min(cus / a.tiles, (d.k + 8191) / 8192);
     info.launches = plan->pieces || a.splits > 1 ? 2 : 1, info.block = 64 * kernel.waves, info.grid = a.tiles * a.splits, info.lds_bytes = kernel.lds;
     const bool walk = kernel.walk && plan->runs;
     if (walk) info.grid = std::min(a.tiles, cus), info.lds_bytes = kernel.walk_lds();
