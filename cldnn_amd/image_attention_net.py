@@ -12,8 +12,9 @@ import numpy as np
 from . import hip, ops
 
 
-def parameters(r, features=64, heads=4, kv_heads=2, blocks=2, patch=8, classes=10):
-    """Random parameters with the factors that keep a signal alive.  r: numpy Generator."""
+def parameters(r, features=64, heads=4, kv_heads=2, blocks=2, patch=8, classes=10, layer_scales=False):
+    """Random parameters with the factors that keep a signal alive.  r: numpy Generator.  layer_scales: a block's two branches have a factor
+    for each feature."""
     d = features // heads
 
     def weights(n, k, scale=1.0):
@@ -35,6 +36,9 @@ def parameters(r, features=64, heads=4, kv_heads=2, blocks=2, patch=8, classes=1
             norm2=norm(), expand=(weights(4 * features, features), vector(4 * features)), contract=(weights(features, 4 * features, 0.5), vector(features))))
     p.update(norm=norm(), kv=(weights(2 * kv_heads * d, features), vector(2 * kv_heads * d)), query=r.standard_normal((heads, d)).astype(np.float32),
              scores=(weights(classes, features), vector(classes)))
+    if layer_scales:
+        for b in p["blocks"]:
+            b.update(scale1=vector(features, 0.7), scale2=vector(features, 0.7))
     return p
 
 
@@ -50,17 +54,9 @@ class ImageAttentionNet:
         rows, qkv = batch * n, (heads + 2 * kv) * d
         self._owned = []
 
-        # patches
-        self.image = hip.Tensor.make("u8", "bfyx", batch, 3, height, width)
-        self._plain, self._blocked = self._keep(hip.Buffer(e, self.image)), self._keep(hip.Buffer(e, hip.Tensor.make("u8", "fs_b_yx_fsv16", batch, 3, height, width)))
-        q = p["patches"]
-        desc = hip.conv_desc(self._blocked.tensor, q["w"].shape, "f32", stride=(patch, patch), bias_dt=hip.F32, has_wqf=True)
-        self._conv = self._keep(hip.Conv(e, desc, q["w"], q["bias"], q["wqf"]))
-        self._patches, self._x = self._keep(hip.Buffer(e, desc.output)), self._keep(hip.Buffer(e, hip.Tensor.make("f32", "byxf", batch, c, y, x)))
+        self._make_patches(height, width)
 
         # one operator per shape: blocks share them, and the buffers between them
-        grid = np.stack(np.meshgrid(np.arange(y), np.arange(x), indexing="ij"), -1).reshape(1, n, 2)
-        self._positions = self._upload(np.broadcast_to(grid, (batch, n, 2)), "i32")
         size = 2
         self._h, self._qkv = self._memory(rows * c * size), self._memory(rows * qkv * size)
         self._o, self._wide = self._memory(rows * c * size), self._memory(rows * 4 * c * size)
@@ -93,6 +89,25 @@ class ImageAttentionNet:
         self._last, self._kv, self._classes = norm(p["norm"]), linear(p["kv"]), linear(p["scores"])
         e.finish()
 
+    def _make_patches(self, height, width):
+        """The int8 convolution from the image to the map, and the patches' positions."""
+        e, p, batch = self.engine, self.params, self.batch
+        c, patch = p["features"], p["patch"]
+        y, x = height // patch, width // patch
+        self.image = hip.Tensor.make("u8", "bfyx", batch, 3, height, width)
+        self._plain, self._blocked = self._keep(hip.Buffer(e, self.image)), self._keep(hip.Buffer(e, hip.Tensor.make("u8", "fs_b_yx_fsv16", batch, 3, height, width)))
+        q = p["patches"]
+        desc = hip.conv_desc(self._blocked.tensor, q["w"].shape, "f32", stride=(patch, patch), bias_dt=hip.F32, has_wqf=True)
+        self._conv = self._keep(hip.Conv(e, desc, q["w"], q["bias"], q["wqf"]))
+        self._patches, self._x = self._keep(hip.Buffer(e, desc.output)), self._keep(hip.Buffer(e, hip.Tensor.make("f32", "byxf", batch, c, y, x)))
+        grid = np.stack(np.meshgrid(np.arange(y), np.arange(x), indexing="ij"), -1).reshape(1, y * x, 2)
+        self._positions = self._upload(np.broadcast_to(grid, (batch, y * x, 2)), "i32")
+
+    def _run_patches(self):
+        hip.reorder(self.engine, self._plain, self._blocked)
+        self._conv.enqueue(self._blocked, self._patches)
+        hip.reorder(self.engine, self._patches, self._x)
+
     def _keep(self, x):
         self._owned.append(x)
         return x
@@ -108,9 +123,7 @@ class ImageAttentionNet:
 
     def enqueue(self):
         """One pass over the image that is in place; nothing is waited for."""
-        hip.reorder(self.engine, self._plain, self._blocked)
-        self._conv.enqueue(self._blocked, self._patches)
-        hip.reorder(self.engine, self._patches, self._x)
+        self._run_patches()
         qkv, x = self._qkv.ptr, self._x
         for b in self._blocks:
             self._norm.enqueue(x, self._h, *b["norm1"])
