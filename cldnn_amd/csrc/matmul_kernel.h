@@ -26,6 +26,7 @@ struct MatmulS8Args : MatmulArgs {
     int32_t a_each, w_each;            // 1: one to a row; 0: one for all
     int32_t out_type, res_type;        // CLDNN_HIP_F32, F16, BF16
     int32_t out_runs;                  // result and residual are whole runs of matmul_run(out_type) values at any place of a tile
+    int32_t past;                      // the result of a large product goes past the caches
 };
 
 // What the kernels ask of an operand's type: a 16-byte piece as the matrix instruction takes it, its sums, the arguments of its product.

@@ -6,6 +6,7 @@
 namespace chip {
 
 constexpr int MATMUL_S8_MOST_K = 131071;  // 128 * 128 of each fit 31 bits
+constexpr int64_t MATMUL_S8_PAST = 64 << 20;
 constexpr int64_t MATMUL_S8_RUN_PITCH = 1 << 20;  // 256 rows of it in f32 are within a buffer's reach
 // Products from which unaligned operands are copied: a launch and two trips of the operands against the kernels for any rows (us, without
 // the copy and with it: 1000 x 401 -> 400 7.1 and 7.9, 1000 x 255 -> 1000 9.2 and 8.1, 1500 x 255 -> 1000 13.0 and 8.4, 20000 x 84 -> 400
@@ -152,7 +153,8 @@ __global__ __launch_bounds__(512, 2) void matmul_s8_walk_kernel(MatmulS8Args a, 
                 vec y;
 #pragma unroll
                 for (int l = 0; l < R; ++l) y[l] = (O)v[k * R + l];
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, y), to, at[k] + i * o_step, 0, 0);
+                if (a.past) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, y), to, at[k] + i * o_step, 0, 2);
+                else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, y), to, at[k] + i * o_step, 0, 0);
             }
         };
         if constexpr (RES) {
@@ -317,6 +319,9 @@ std::unique_ptr<OperatorPlan> matmul_s8_plan(const cldnn_hip_engine_s& e, const 
     a.bias = mark(d.has_bias), a.residual = mark(res_size);
     const auto runs = [&](int64_t pitch) { return pitch % matmul_s8_run(a) == 0 && pitch <= MATMUL_S8_RUN_PITCH; };
     plan->runs = a.n % matmul_s8_run(a) == 0 && runs(a.o_pitch) && (!a.residual || runs(a.r_pitch));
+    // A result larger than the dies' caches together leaves them to the operands: 25088 x 1024 -> 4096, 196 MiB, 140 and 134 us; 25088 x 4096 ->
+    // 1024, 49 MiB, is the same either way.
+    a.past = (int64_t)d.m * d.n * out_size >= MATMUL_S8_PAST;
     const int cus = plan->cus = e.props.multiProcessorCount;
     const bool whole = d.k % 16 == 0 && a.a_pitch % 16 == 0 && a.w_pitch % 16 == 0 && std::max(a.a_pitch, a.w_pitch) < (1 << 22);
     plan->kernel = choose(d.m, d.n, d.k, whole, cus);

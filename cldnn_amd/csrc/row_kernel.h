@@ -11,6 +11,7 @@ namespace chip {
 // Values of the longest row: 512 threads leave 256 registers to each, which 8 vectors of two tensors of f32 and the values made of them fit
 // (1024 threads with 4 vectors each, in 128 registers, keep some in scratch memory).
 constexpr int ROW_MOST = 8 * 512 * 8;
+constexpr int64_t ROW_PAST = 32 << 20;  // bytes that the dies' caches hold together
 
 // Waves of a SIMD that a kernel with NV vectors a lane leaves registers for: what covers a row's trips to memory is other rows.
 constexpr int row_waves(int NV) { return NV == 1 ? 7 : NV == 2 ? 6 : NV == 3 ? 4 : NV == 4 ? 3 : 2; }
@@ -108,7 +109,15 @@ __device__ __forceinline__ void row_values(const RowRaw<WIDE>& x, int type, floa
 
 __device__ __forceinline__ void row_floats(const float* row, int c, int C, float (&v)[8]) { row_values(row_load<true>(row, CLDNN_HIP_F32, c, C), CLDNN_HIP_F32, v); }
 
-template <typename T>
+// PAST: past the caches
+template <bool PAST, typename V, typename A>
+__device__ __forceinline__ void row_write(A* p, const V& x)
+{
+    if constexpr (PAST) __builtin_nontemporal_store((A)x, p);
+    else *p = x;
+}
+
+template <bool PAST, typename T>
 __device__ __forceinline__ void row_store_as(T* row, const RowVector& of, int C, const float (&v)[8])
 {
     typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
@@ -121,7 +130,7 @@ __device__ __forceinline__ void row_store_as(T* row, const RowVector& of, int C,
             vec x;
 #pragma unroll
             for (int i = 0; i < W; ++i) x[i] = (T)v[W * j + i];
-            ((any*)p)[j] = x;
+            row_write<PAST>((any*)p + j, x);
         }
     } else if (of.from < 8) {
 #pragma unroll
@@ -131,11 +140,12 @@ __device__ __forceinline__ void row_store_as(T* row, const RowVector& of, int C,
 }
 
 // rounded once, to the type
+template <bool PAST>
 __device__ __forceinline__ void row_store(void* row, int type, const RowVector& of, int C, const float (&v)[8])
 {
-    if (type == CLDNN_HIP_F32) row_store_as((float*)row, of, C, v);
-    else if (type == CLDNN_HIP_F16) row_store_as((_Float16*)row, of, C, v);
-    else row_store_as((__bf16*)row, of, C, v);
+    if (type == CLDNN_HIP_F32) row_store_as<PAST>((float*)row, of, C, v);
+    else if (type == CLDNN_HIP_F16) row_store_as<PAST>((_Float16*)row, of, C, v);
+    else row_store_as<PAST>((__bf16*)row, of, C, v);
 }
 
 // ----------------------------------------------------------------------------- over a row

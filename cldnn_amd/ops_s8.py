@@ -181,7 +181,11 @@ class BlockNorm(Operator):
 
     def enqueue(self, x, y=None, out=None, *, branch=None, post_weight=None, post_bias=None, gate=None, weight=None, bias=None, scale=None, shift=None, out_scales=None):
         """y: the stream behind the block, which may be x itself; None: not wanted."""
-        given = (x, branch, post_weight, post_bias, gate, weight, bias, scale, shift, y, out, out_scales)
-        status = self._enqueue(self.h, *[of(g) for of, g in zip(self._address, given)])
+        of = self._address
+        # what is not given, most of it in most calls, is not asked for: 0.4 us of 5.2
+        status = self._enqueue(
+            self.h, of[0](x), None if branch is None else of[1](branch), None if post_weight is None else of[2](post_weight), None if post_bias is None else of[3](post_bias),
+            None if gate is None else of[4](gate), None if weight is None else of[5](weight), None if bias is None else of[6](bias), None if scale is None else of[7](scale),
+            None if shift is None else of[8](shift), None if y is None else of[9](y), None if out is None else of[10](out), None if out_scales is None else of[11](out_scales))
         if status:
             hip.check(status)

@@ -167,6 +167,12 @@ def test_many_tokens(eng):
     check(eng, 3001, 1024, "bf16", branch="bf16", out="bf16", modulation="bf16", per_image=1000)
 
 
+@pytest.mark.parametrize("out", ["f32", "f16", "s8"])
+def test_results_that_go_past_the_caches(eng, out):
+    # 34 MiB each; a last vector that lies over the one before it; in place
+    check(eng, 8501, 1052, "f32", branch="f16", out=out, norm="layer", in_place=out == "s8")
+
+
 @pytest.mark.parametrize("features", [84, 1024, 4100, 12000])
 def test_a_mean_far_from_zero_costs_no_digits(eng, features):
     # the squares are taken around the mean: a deviation of 1 at a mean of 1000 keeps what the mean leaves of 32 bits
