@@ -18,6 +18,9 @@ constexpr int64_t MATMUL_S8_PACK = 200ll << 20;
 // is the end of a tile.  The next tile's first operands are asked for in front of it, and its stores drain under the next one's products,
 // where a workgroup to a tile waits for all of them before its LDS is free for the next.  Scales and bias are asked for a tile ahead,
 // a value to a thread, and handed out through LDS; every place of the result is an offset that is worked out once.
+// Bound by the matrix cores at the power limit, and by the end of a tile in the vector units (8192 x 8192 x 8192 419 us, 2.63 POP/s,
+// the matrix cores 63 % of the time busy at 1.97 GHz; 25088 x 1024 -> 4096 with a gelu, eight steps of K to a tile and seven rounds of tiles,
+// 134 us, 1.57 POP/s; 25088 x 4096 -> 1024 with a residual 104 us, 2.0).
 // O: the result's type; RES: a residual is added.  The result (and the residual) is whole runs (MatmulS8Args::out_runs).
 template <typename O, bool RES, int MB>
 __global__ __launch_bounds__(512, 2) void matmul_s8_walk_kernel(MatmulS8Args a, const int8_t* x, const int8_t* w, void* out)
@@ -262,9 +265,11 @@ int choose(int m, int n, int k, bool whole, int cus)
     const auto tiles = [&](int row) { return count(m, n, matmul_s8_kernels[row]); };
     // Few tiles of any size: the smallest, whose eight waves split K.  (us, against 32 x 64 tiles: 32 x 256 -> 4096, 512 of them, 4.4 and 6.0,
     // 32 x 1024 -> 4096 5.3 and 6.5, 1 x 4096 -> 8192 8.6 and 10.5; every one reads all of its rows, so not many with a long K: 784 x 4096
-    // -> 96, 294 of them, 10.5 and 9.0)
+    // -> 96, 294 of them, 10.5 and 9.0.  With more than 8 rows over a long K they are not more than the CUs where there is a choice: 16 x 8192
+    // -> 5120, 320 of them, 17.7 and 13.5, 16 x 4096 -> 5120 10.7 and 9.4, 8 x 4096 -> 5120 9.4 and 9.3, 16 x 3008 -> 5120 7.4 and 8.4.)
     const int64_t few = tiles(MM_16);
-    if (few <= (k <= 512 ? 3 * cus : k <= 1024 || m <= 16 ? 2 * cus : k <= 2048 || m <= 64 ? cus * 5 / 4 : cus)) return MM_16;
+    const bool heavy = whole && m > 8 && m <= 16 && k >= 4096;
+    if (few <= (k <= 512 ? 3 * cus : heavy ? cus : k <= 1024 || m <= 16 ? 2 * cus : k <= 2048 || m <= 64 ? cus * 5 / 4 : cus)) return MM_16;
     if (!whole) return tiles(MM_ANY_64) >= cus ? MM_ANY_64 : MM_ANY_32;
     int best = MM_32;
     double least = 1e30;

@@ -147,6 +147,7 @@ def test_scales_that_are_no_number_stay_in_their_rows(eng, size):
 KERNELS = [
     ((4090, 4093, 144), "tile<256x256>"), ((7160, 2042, 272), "tile<224x256>"), ((6130, 2046, 64), "tile<192x256>"), ((4090, 4092, 144), "walk<256x256>"), ((7160, 2040, 272), "walk<224x256>"), ((6130, 2044, 64), "walk<192x256>"), ((3100, 1537, 208), "tile<128x128>"),
     ((1601, 1000, 112), "tile<64x128>"), ((1001, 1000, 272), "tile<64x64,k2>"), ((190, 2000, 528), "tile<32x64,k4>"), ((30, 1000, 1000), "split<16x16>"),
+    ((16, 4200, 4096), "tile<32x64,k4>"), ((8, 4200, 4096), "split<16x16>"), ((13, 4200, 4160), "tile<32x64,k4>"), ((16, 4200, 2112), "split<16x16>"),
     ((7, 250, 18000), "split<16x16> + matmul_join"), ((1, 31, 16383), "split<16x16> + matmul_join"), ((20, 65, 18200), "split<16x16> + matmul_join"),
     ((1001, 1000, 255), "tile<64x64,k2>"), ((600, 500, 63), "split<32x32>"), ((1601, 1400, 61), "split<64x64>"), ((1601, 1000, 263), "tile<64x128>"), ((3101, 1700, 263), "tile<128x128>")]
 
