@@ -3,9 +3,9 @@
  * cldnn_hip_ops.h: rows quantised with a scale each, the matrix product of int8 operands with scales for each token and channel,
  * and the norms before and after a block with its gate and residual scale, whose result may be int8 too.
  *
- * The reference has none of them.  Objects, scratch memory, streams, recordings, threads and errors are those of cldnn_hip_ops.h, and
- * cldnn_hip_operator_retain, _release and _get_info serve these objects as well.  Exported by libcldnn_hip_ops_s8.so, which needs
- * libcldnn_hip_ops.so and libcldnn_hip.so.
+ * The reference has none of them.  Objects, scratch memory, streams, recordings, threads, errors, alignment and overlap are as in
+ * cldnn_hip_ops.h, and cldnn_hip_operator_retain, _release and _get_info serve these objects as well.  Exported by
+ * libcldnn_hip_ops_s8.so, which needs libcldnn_hip_ops.so and libcldnn_hip.so.
  *
  * A quantised row: 8-bit whole numbers q and one float, scale; the values it stands for are q * scale.  Of values y it is
  *   most = max |y|,   scale = most / 127,   q = y * (127 / most) rounded to the nearest whole number, ties to even,
