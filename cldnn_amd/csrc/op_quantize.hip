@@ -1,8 +1,8 @@
 // Rows to int8 with a scale each: q = rint(y * (127 / max |y|)), y = act(x) * factor, or act(x) * gate * factor.
 //
 // A row is read once and held in registers between its maximum and its values.  25088 x 4096 in f16, 308 MB: 52 us, 5.9 TB/s of what is partly
-// in the caches; behind a gelu 73 us, its exponential and reciprocal at a quarter of the rate of the vector units, which nothing overlaps
-// but the other rows of the CU.
+// in the caches; behind a gelu 73 us: its 12 instructions to a value, the exponential at a quarter of the rate, keep the vector units as
+// long as the rows' trips to memory take, and three waves of a SIMD overlap the two in part.
 #include "row_kernel.h"
 
 namespace chip {
