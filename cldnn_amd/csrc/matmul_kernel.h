@@ -13,19 +13,23 @@ struct MatmulArgs {
     const float* bias;
     const void* residual;  // nullptr: none
     Act act, act2;
-    int32_t res_float, out_float;
     int32_t tiles, tiles_m, tiles_n;  // of the result
     int32_t band;                     // rows of tiles in a band
     int32_t splits;                   // workgroups that split K for each tile: their sums go to part[split][m][n]
     void* part;                       // of the operands' sums: float or int32_t
 };
 
-// ... and of the product of int8 operands: scales of the rows of a and of the weights' rows, out types apart from the operands'
+// ... of the product of float operands: result and residual are of their type or f32
+struct MatmulFloatArgs : MatmulArgs {
+    int32_t res_float, out_float;
+};
+
+// ... and of int8 operands: scales of the rows of a and of the weights' rows, out types apart from the operands'
 struct MatmulS8Args : MatmulArgs {
     const float *a_scales, *w_scales;  // nullptr: 1
     int32_t a_each, w_each;            // 1: one to a row; 0: one for all
     int32_t out_type, res_type;        // CLDNN_HIP_F32, F16, BF16
-    int32_t out_runs;                  // result and residual are whole runs of matmul_run(out_type) values at any place of a tile
+    int32_t out_runs;                  // result and residual are whole runs of matmul_run values at any place of a tile
     int32_t past;                      // the result of a large product goes past the caches
 };
 
@@ -37,7 +41,7 @@ template <typename T> struct MatmulType {
     typedef v4i_any Any;  // a piece at any element's address
     typedef v4f Sum;
     typedef float One;
-    typedef MatmulArgs Args;
+    typedef MatmulFloatArgs Args;
     static constexpr int E = 8;  // values of a piece
     static constexpr bool SHORT = false;  // form of the activations
 };
@@ -119,7 +123,7 @@ __device__ __forceinline__ void matmul_write(O* p, int valid, const V (&v)[N])
 
 // N neighbouring features from n0 on of row m behind their activation: the residual, the result
 template <typename T, int N>
-__device__ __forceinline__ void matmul_write_row(const MatmulArgs& a, float (&v)[N], int m, int n0, void* out)
+__device__ __forceinline__ void matmul_write_row(const MatmulFloatArgs& a, float (&v)[N], int m, int n0, void* out)
 {
     const int valid = a.n - n0;
     if (m >= a.m || valid <= 0) return;
@@ -337,10 +341,10 @@ __global__ __launch_bounds__(256) void matmul_join_kernel(typename MatmulType<T>
 }
 
 // ----------------------------------------------------------------------------- the end of a tile of int8 operands
-// Values of a run: 16 bytes of the result, which a lane stores as one piece beside those of its neighbours.  Four lanes write 64 bytes
-// without a gap then; 16 neighbours to a lane, as the float products have them, are written in pieces 32 bytes apart, and 25088 x 1024 ->
-// 4096 took twice the requests to memory.
-__device__ inline int matmul_run(int type) { return type == CLDNN_HIP_F32 ? 4 : 8; }
+// Values of a run, of results of `size` bytes: 16 bytes, which a lane stores as one piece beside those of its neighbours.  Four lanes write
+// 64 bytes without a gap then; 16 neighbours to a lane, as the float products have them, are written in pieces 32 bytes apart, and 25088 x
+// 1024 -> 4096 took twice the requests to memory.
+constexpr int matmul_run(int size) { return 16 / size; }
 
 // Where the g-th four of a lane's 16 values lie among the wave's 64 features.
 __device__ inline int matmul_four(const MatmulS8Args& a, int g, int q) { return a.out_type == CLDNN_HIP_F32 ? 16 * g + 4 * q : 32 * (g >> 1) + 8 * q + 4 * (g & 1); }
@@ -441,7 +445,7 @@ __device__ __forceinline__ void matmul_finish_s8(const MatmulS8Args& a, const v4
         if (runs) {
             matmul_typed(a.out_type, [&](auto t) {
                 typedef decltype(t) T;
-                constexpr int R = 16 / sizeof(T);
+                constexpr int R = matmul_run(sizeof(T));
                 typedef T vec __attribute__((ext_vector_type(R)));
 #pragma unroll
                 for (int l = 0; l < 16; l += R) {
@@ -463,7 +467,7 @@ __device__ __forceinline__ void matmul_finish_s8(const MatmulS8Args& a, const v4
 
 // The sums of a wave, 16 MB rows from m on x 64 features from n on, of float operands: bias, activation, residual, the result.
 template <typename T, int MB>
-__device__ __forceinline__ void matmul_finish_rows(const MatmulArgs& a, const v4f (&sum)[4][MB], int m, int n, int lane, void* out)
+__device__ __forceinline__ void matmul_finish_rows(const MatmulFloatArgs& a, const v4f (&sum)[4][MB], int m, int n, int lane, void* out)
 {
     const int q = lane >> 4, r = lane & 15;
     n += 16 * q;

@@ -6,7 +6,7 @@ namespace chip {
 constexpr int64_t MATMUL_PACK = 200ll << 20;  // products from which unaligned operands are copied
 
 struct MatmulPlan {
-    MatmulArgs a;
+    MatmulFloatArgs a;
     int dt;
     int kernel;  // row of matmul_kernels; the one for any strides where pointers are not aligned
     int any;
@@ -76,7 +76,7 @@ MatmulPlan* matmul_plan(const cldnn_hip_engine_s& e, const cldnn_hip_matmul_desc
     CHIP_REQUIRE(d.residual_dtype != CLDNN_HIP_NO_TYPE || d.residual_activation == CLDNN_HIP_ACT_NONE, CLDNN_HIP_INVALID_ARG,
                  "matmul: an activation of the sum without a residual");
     std::unique_ptr<MatmulPlan> plan(new MatmulPlan{});
-    MatmulArgs& a = plan->a;
+    MatmulFloatArgs& a = plan->a;
     a.m = d.m, a.n = d.n, a.k = d.k;
     const auto pitch = [](int64_t stride, int64_t dense) {
         CHIP_REQUIRE(stride == 0 || stride >= dense, CLDNN_HIP_INVALID_ARG, "matmul: a stride shorter than its row");
@@ -120,7 +120,7 @@ MatmulPlan* matmul_plan(const cldnn_hip_engine_s& e, const cldnn_hip_matmul_desc
 
 void matmul_launch(hipStream_t s, const MatmulPlan& p, void* workspace, const void* x, const void* w, const float* bias, const void* residual, void* out)
 {
-    MatmulArgs a = p.a;
+    MatmulFloatArgs a = p.a;
     CHIP_REQUIRE((!a.bias || bias) && (!a.residual || residual), CLDNN_HIP_INVALID_ARG, "null device pointer");
     check_aligned(x, 2, "a"), check_aligned(w, 2, "weights"), check_aligned(out, a.out_float ? 4 : 2, "output");
     if (a.bias) check_aligned(bias, 4, "bias"), a.bias = bias;

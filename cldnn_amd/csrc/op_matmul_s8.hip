@@ -27,7 +27,7 @@ __global__ __launch_bounds__(512, 2) void matmul_s8_walk_kernel(MatmulS8Args a, 
 {
     constexpr int WN = 4, WAVES = 8, BM = 32 * MB, BN = 256, BK = 128;
     constexpr int XL = (BM / 8 + WAVES - 1) / WAVES, WL = BN / 8 / WAVES;  // loads of a wave: 8 rows each
-    constexpr int R = 16 / sizeof(O), RUNS = 16 / R;
+    constexpr int R = matmul_run(sizeof(O)), RUNS = 16 / R;
     __shared__ v4i lds[2 * (BM + BN) * 8];
     __shared__ float rows[BM], columns[2 * BN];  // of the tile that ends: scales of rows; scales of features, bias
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -282,8 +282,6 @@ int choose(int m, int n, int k, bool whole, int cus)
     return best;
 }
 
-int matmul_s8_run(const MatmulS8Args& a) { return a.out_type == CLDNN_HIP_F32 ? 4 : 8; }
-
 void set_tiles(MatmulS8Args& a, const MatmulS8Kernel& k)
 {
     const int64_t tiles = count(a.m, a.n, k);
@@ -322,8 +320,9 @@ std::unique_ptr<OperatorPlan> matmul_s8_plan(const cldnn_hip_engine_s& e, const 
     const auto mark = [](bool has) { return has ? (const float*)4 : nullptr; };
     a.a_scales = mark(d.a_scales != CLDNN_HIP_SCALES_NONE), a.w_scales = mark(d.weights_scales != CLDNN_HIP_SCALES_NONE);
     a.bias = mark(d.has_bias), a.residual = mark(res_size);
-    const auto runs = [&](int64_t pitch) { return pitch % matmul_s8_run(a) == 0 && pitch <= MATMUL_S8_RUN_PITCH; };
-    plan->runs = a.n % matmul_s8_run(a) == 0 && runs(a.o_pitch) && (!a.residual || runs(a.r_pitch));
+    const int run = matmul_run((int)out_size);
+    const auto runs = [&](int64_t pitch) { return pitch % run == 0 && pitch <= MATMUL_S8_RUN_PITCH; };
+    plan->runs = a.n % run == 0 && runs(a.o_pitch) && (!a.residual || runs(a.r_pitch));
     // A result larger than the dies' caches together leaves them to the operands: 25088 x 1024 -> 4096, 196 MiB, 140 and 134 us; 25088 x 4096 ->
     // 1024, 49 MiB, is the same either way.
     a.past = (int64_t)d.m * d.n * out_size >= MATMUL_S8_PAST;
@@ -366,7 +365,7 @@ void matmul_s8_launch(hipStream_t s, const OperatorPlan& plan, void* workspace, 
     if (a.w_scales) check_aligned(w_scales, 4, "weights_scales"), a.w_scales = w_scales;
     if (a.bias) check_aligned(bias, 4, "bias"), a.bias = bias;
     if (a.residual) check_aligned(residual, float_size(a.res_type, ""), "residual"), a.residual = residual;
-    const auto whole = [&](const void* p, int type) { return ((uintptr_t)p & (std::min(16, matmul_s8_run(a) * float_size(type, "")) - 1)) == 0; };
+    const auto whole = [&](const void* p, int type) { return ((uintptr_t)p & (std::min(16, matmul_run(float_size(a.out_type, "")) * float_size(type, "")) - 1)) == 0; };
     a.out_runs = p.runs && whole(out, a.out_type) && (!a.residual || whole(residual, a.res_type));
     const int8_t *xa = (const int8_t*)x, *wa = (const int8_t*)w;
     a.part = workspace;
