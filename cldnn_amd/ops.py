@@ -209,8 +209,13 @@ class Buffer:
 
 
 def to_type(values, dtype):
-    """numpy array of the bits of `values` in an operator's type; bf16, which numpy has not, as uint16 rounded to nearest even"""
+    """numpy array of the bits of `values` in an operator's type; bf16, which numpy has not, as uint16 rounded to nearest even; s8: rounded to
+    the nearest whole number, ties to even, and held to -128 .. 127, NaN as 0"""
     dt = _type(dtype)
+    if dt == hip.S8:
+        values = np.asarray(values)
+        if values.dtype != np.int8:
+            values = np.clip(np.rint(np.nan_to_num(values, nan=0.0, posinf=127, neginf=-128)), -128, 127)
     if dt == BF16:
         with np.errstate(over="ignore"):
             single = np.ascontiguousarray(values, np.float32)
