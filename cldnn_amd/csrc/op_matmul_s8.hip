@@ -282,10 +282,10 @@ int choose(int m, int n, int k, bool whole, int cus)
     return best;
 }
 
-void set_tiles(MatmulS8Args& a, const MatmulS8Kernel& k)
+void set_tiles(MatmulS8Args& a, const MatmulS8Kernel& k, const char* what)
 {
     const int64_t tiles = count(a.m, a.n, k);
-    check_grid(tiles, 64 * k.waves, "matmul s8");
+    check_grid(tiles, 64 * k.waves, what);
     a.tiles = (int32_t)tiles, a.tiles_m = (a.m + k.rows - 1) / k.rows, a.tiles_n = (a.n + k.features - 1) / k.features;
     a.band = 8;
 }
@@ -335,7 +335,7 @@ std::unique_ptr<OperatorPlan> matmul_s8_plan(const cldnn_hip_engine_s& e, const 
         plan->kernel = choose(d.m, d.n, d.k, true, cus);
     }
     const MatmulS8Kernel& kernel = matmul_s8_kernels[plan->kernel];
-    set_tiles(a, kernel);
+    set_tiles(a, kernel, "matmul s8");
     // The smallest tiles that leave half of the chip idle over a long K: workgroups that take 8192 of it each, a run of loads of their waves,
     // for the price of a second launch (us, one workgroup and several: 16 x 25088 -> 1000 24.9 and 13.8, 16 x 16384 -> 1000 17.0 and 13.1,
     // 1 x 16384 -> 500 11.6 and 9.9; 1 x 12288 -> 500 9.5 and 9.8; more and shorter parts gain nothing).
@@ -376,7 +376,7 @@ void matmul_s8_launch(hipStream_t s, const OperatorPlan& plan, void* workspace, 
     }
     const int row = (((uintptr_t)xa | (uintptr_t)wa) & 15) == 0 ? p.kernel : p.any;
     const MatmulS8Kernel& kernel = matmul_s8_kernels[row];
-    set_tiles(a, kernel);
+    set_tiles(a, kernel, row == p.kernel ? "matmul s8" : "matmul s8, operands that are not aligned to 16 bytes");
     const auto launch = [&](auto f) { hipLaunchKernelGGL(f, dim3(kernel.walk && a.out_runs ? std::min(a.tiles, p.cus) : a.tiles, a.splits), dim3(64 * kernel.waves), 0, s, a, xa, wa, out); };
     const auto large = [&](auto mb) {
         constexpr int MB = decltype(mb)::value;

@@ -42,7 +42,9 @@ cldnn_hip_status cldnn_hip_quantize_enqueue(cldnn_hip_operator op, const void* i
 /* ------------------------------------------------------------------ matrix product of int8 operands
  *   out[i][j] = act2(act(sum_k a[i][k] * weights[j][k] * a_scale[i] * weights_scale[j] + bias[j]) + residual[i][j])
  * a: m rows of k int8, weights: n rows of k int8.  The sum is exact; it is rounded to 32 bits, multiplied by the row's scale, then by the
- * channel's, and the result rounded once at the end.  The residual may lie in the output (same pointer, stride and type). */
+ * channel's, and the result rounded once at the end.  The residual may lie in the output (same pointer, stride and type).
+ * Operands that are not aligned to 16 bytes take smaller tiles: enqueue refuses them (CLDNN_HIP_UNSUPPORTED_SIZE) where the result has
+ * 2^24 tiles of 64 x 64 or more. */
 enum {
     CLDNN_HIP_SCALES_NONE = 0,        /* 1 */
     CLDNN_HIP_SCALES_ONE = 1,         /* one for all rows */
