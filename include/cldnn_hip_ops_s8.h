@@ -11,6 +11,9 @@
  *   most = max |y|,   scale = most / 127,   q = y * (127 / most) rounded to the nearest whole number, ties to even,
  * each quotient and product rounded to 32 bits; |q| <= 127.  A row whose `most` is below 2^-120 counts as zeros (scale 0).  A row with
  * a NaN or an infinity gets q = 0 and scale NaN, so that every product of the row is NaN.
+ *
+ * CLDNN_HIP_ACT_GELU is worked out to within 1.5e-7 |v|, which far below zero may be as much as the value: a row of nothing but such v
+ * becomes the quantised row of what was worked out.
  */
 #ifndef CLDNN_HIP_OPS_S8_H
 #define CLDNN_HIP_OPS_S8_H
