@@ -3,7 +3,8 @@
 //
 // One pass: a token's row is read once and held in registers; the mean is taken first, then the squares around it, so that a mean far
 // from zero costs no digits.  Bound by memory: 25088 x 1024 in bf16, a branch with gate, scale and shift, 206 MB, 44 us, 4.7 TB/s; 784 x
-// 8192 of an f32 stream with an f16 branch, norms on both sides, 77 MB, 16.6 us, 4.6 TB/s.  One token takes a launch, 3 us.
+// 8192 of an f32 stream with an f16 branch, norms on both sides, 77 MB, 16.6 us, 4.6 TB/s.  Narrow rows, 16 threads to each, 12 of which have
+// a vector: 100352 x 96 in bf16, as the first, 77 MB, 21 us, 3.7 TB/s; 100352 x 128, 103 MB, 22 us, 4.7.  One token takes a launch, 3 us.
 #include "row_kernel.h"
 
 namespace chip {

@@ -6,7 +6,7 @@
 namespace chip {
 
 constexpr int MATMUL_S8_MOST_K = 131071;  // 128 * 128 of each fit 31 bits
-constexpr int64_t MATMUL_S8_PAST = 64 << 20;
+constexpr int64_t MATMUL_S8_PAST = 64 << 20;  // twice what the dies' caches hold together
 constexpr int64_t MATMUL_S8_RUN_PITCH = 1 << 20;  // 256 rows of it in f32 are within a buffer's reach
 // Products from which unaligned operands are copied: a launch and two trips of the operands against the kernels for any rows (us, without
 // the copy and with it: 1000 x 401 -> 400 7.1 and 7.9, 1000 x 255 -> 1000 9.2 and 8.1, 1500 x 255 -> 1000 13.0 and 8.4, 20000 x 84 -> 400
@@ -18,9 +18,9 @@ constexpr int64_t MATMUL_S8_PACK = 200ll << 20;
 // is the end of a tile.  The next tile's first operands are asked for in front of it, and its stores drain under the next one's products,
 // where a workgroup to a tile waits for all of them before its LDS is free for the next.  Scales and bias are asked for a tile ahead,
 // a value to a thread, and handed out through LDS; every place of the result is an offset that is worked out once.
-// Bound by the matrix cores at the power limit, and by the end of a tile in the vector units (8192 x 8192 x 8192 419 us, 2.63 POP/s,
-// the matrix cores 63 % of the time busy at 1.97 GHz; 25088 x 1024 -> 4096 with a gelu, eight steps of K to a tile and seven rounds of tiles,
-// 134 us, 1.57 POP/s; 25088 x 4096 -> 1024 with a residual 104 us, 2.0).
+// Bound by the matrix cores at the power limit, and by the end of a tile in the vector units (on several cards, 8192 x 8192 x 8192 419 to
+// 445 us, 2.47 to 2.63 POP/s, the matrix cores 63 % of the time busy at 1.97 GHz; 25088 x 1024 -> 4096 with a gelu, eight steps of K to a tile
+// and seven rounds of tiles, 127 to 136 us, 1.55 to 1.66 POP/s; 25088 x 4096 -> 1024 with a residual 104 to 117 us, 1.8 to 2.0).
 // O: the result's type; RES: a residual is added.  The result (and the residual) is whole runs (MatmulS8Args::out_runs).
 template <typename O, bool RES, int MB>
 __global__ __launch_bounds__(512, 2) void matmul_s8_walk_kernel(MatmulS8Args a, const int8_t* x, const int8_t* w, void* out)
@@ -249,7 +249,8 @@ int64_t count(int m, int n, const MatmulS8Kernel& k) { return (int64_t)((m + k.r
 
 // What a kernel takes in us behind a launch: for each round that its tiles need on the chip, base + step * K, measured over 324 sizes of 1 to
 // 25088 rows, 96 to 8192 features and K of 256 to 16384 (f16 results).  Of two workgroups to a CU a full round has both, and a last
-// one of at most one to a CU has the `one` figures.  The kernel with the least sum was the best or within 6 % of it.
+// one of at most one to a CU has the `one` figures.  The kernel with the least sum was the best at 315 of them and at most 7 % behind it
+// at the others (profiles/operators_s8_kernel_choice.txt).
 struct MatmulS8Time {
     int kernel, on_cu;  // workgroups to a CU
     double base, step, one_base, one_step;
@@ -323,8 +324,10 @@ std::unique_ptr<OperatorPlan> matmul_s8_plan(const cldnn_hip_engine_s& e, const 
     const int run = matmul_run((int)out_size);
     const auto runs = [&](int64_t pitch) { return pitch % run == 0 && pitch <= MATMUL_S8_RUN_PITCH; };
     plan->runs = a.n % run == 0 && runs(a.o_pitch) && (!a.residual || runs(a.r_pitch));
-    // A result larger than the dies' caches together leaves them to the operands: 25088 x 1024 -> 4096, 196 MiB, 140 and 134 us; 25088 x 4096 ->
-    // 1024, 49 MiB, is the same either way.
+    // A result of twice the dies' caches leaves them to the operands (us, through them and past them: behind a gelu 25088 x 1024 -> 4096, 196 MiB,
+    // 138 and 130, 25088 x 512 -> 2048, 98 MiB, 57.1 and 53.5, 16384 x 1024 -> 2048, 64 MiB, 44.5 and 44.9; without one, in the same order, 122
+    // and 118, 46.6 and 48.6, 40.8 and 46.9).  Half as large, a gelu's results gain 2 us of 24 to 38 and others lose as much (25088 x 1024 -> 1024,
+    // 49 MiB, 38.5 and 37.4, 33.3 and 35.7).
     a.past = (int64_t)d.m * d.n * out_size >= MATMUL_S8_PAST;
     const int cus = plan->cus = e.props.multiProcessorCount;
     const bool whole = d.k % 16 == 0 && a.a_pitch % 16 == 0 && a.w_pitch % 16 == 0 && std::max(a.a_pitch, a.w_pitch) < (1 << 22);
